@@ -12,9 +12,10 @@ A case is one call of one operator.  `kind`:
 "gate_up"  add, RMSNorm, 8-bit rows, the product with a stacked gate/up weight [2 N, K] and
            silu(gate) * up: what stands in front of a feed-forward's second product.
 
-The 4-bit form: a group is up to 64 neighbouring elements of a head of one token; lo is its
-smallest element rounded down to bfloat16, step a fifteenth of the way from there to its largest
-in float16, and an element is held as the nearest of lo + step * (0 .. 15).  The 8-bit form: a
+The 4-bit form: a group is up to 64 neighbouring elements of a head of one token; its step is a
+fifteenth of the way from its smallest element (or zero, if that is less) to its largest (or
+zero) in float16, its zero the whole number of steps nearest to that way's share below zero, and
+an element is held as the nearest of step * (0 - zero .. 15 - zero).  The 8-bit form: a
 row's scale is its largest magnitude / 127, an element the nearest whole number of scales.
 """
 
@@ -215,34 +216,25 @@ EPS = 1e-6
 # ------------------------------------------------------------------ plain forms
 
 
-def _down_to_bf16(x):
-    """float32 -> the largest bfloat16 not above it."""
-    bits = x.float().view(torch.int32)
-    cut = bits & -65536
-    cut = torch.where((bits < 0) & (cut != bits), cut + 65536, cut)
-    return cut.view(torch.float32).to(torch.bfloat16)
-
-
 def _quantize4(x):
-    """[..., dim] -> codes [..., dim] (uint8), step and lo [..., groups]."""
+    """[..., dim] -> codes [..., dim] (uint8), step (float16) and zero [..., groups]."""
     dim, n = x.shape[-1], _groups(x.shape[-1])
-    wide = torch.nn.functional.pad(x.float(), (0, n * GROUP - dim), value=float("nan"))
-    wide = wide.unflatten(-1, (n, GROUP))
-    real = ~wide.isnan()
-    least = wide.where(real, wide.new_full((), math.inf)).amin(-1)
-    most = wide.where(real, wide.new_full((), -math.inf)).amax(-1)
-    lo = _down_to_bf16(least)
-    step = ((most - lo.float()) / torch.full((), 15.0, device=x.device)).clamp(max=65504.0).half()
+    # (zeros fill the last group up: zero is among what every group spans)
+    wide = torch.nn.functional.pad(x.float(), (0, n * GROUP - dim)).unflatten(-1, (n, GROUP))
+    least, most = wide.amin(-1).clamp(max=0.0), wide.amax(-1).clamp(min=0.0)
+    step = ((most - least) / torch.full((), 15.0, device=x.device)).clamp(max=65504.0).half()
     # the border between two codes is decided in 64 bits
-    c = (wide.double() - lo.double()[..., None]) / step.double()[..., None].clamp(min=1e-30)
-    c = c.where(step[..., None] > 0, torch.zeros_like(c)).round().clamp(0, 15)
-    return c.flatten(-2)[..., :dim].to(torch.uint8), step, lo
+    by = step.double().where(step > 0, torch.ones((), dtype=torch.double, device=x.device))
+    zero = (-least.double() / by).round().clamp(max=15).where(step > 0, by - by)
+    c = (wide.double() / by[..., None]).round() + zero[..., None]
+    c = c.clamp(0, 15).where(step[..., None] > 0, c - c)
+    return c.flatten(-2)[..., :dim].to(torch.uint8), step, zero.to(torch.uint8)
 
 
-def _values4(codes, step, lo):
+def _values4(codes, step, zero):
     dim = codes.shape[-1]
     s = step.float().repeat_interleave(GROUP, -1)[..., :dim]
-    return lo.float().repeat_interleave(GROUP, -1)[..., :dim] + s * codes.float()
+    return s * (codes.float() - zero.float().repeat_interleave(GROUP, -1)[..., :dim])
 
 
 def _quantize8(x):
@@ -378,7 +370,7 @@ def prepare(case, seed):
     for name in ("keys", "values"):
         s[name] = (torch.zeros(num_pages, kv, P, dim, dtype=torch.uint8, device=DEVICE),
                    torch.zeros(num_pages, kv, P, n, dtype=torch.half, device=DEVICE),
-                   torch.zeros(num_pages, kv, P, n, dtype=torch.bfloat16, device=DEVICE))
+                   torch.zeros(num_pages, kv, P, n, dtype=torch.uint8, device=DEVICE))
     if case["kind"] == "store":
         s["pages"], s["slots"] = _places(requests, table, P)
         return s
@@ -419,18 +411,15 @@ def _nearest4(x):
     out = x.double()
     for a in range(0, x.shape[-1], GROUP):
         part = x[..., a:a + GROUP].double()
-        least, most = part.min(-1, keepdim=True)[0], part.max(-1, keepdim=True)[0]
-        lo = least.bfloat16().double()
-        # one bfloat16 down where rounding went up
-        gap = torch.where(lo == 0, torch.full_like(lo, 2.0 ** -133),
-                          2.0 ** (torch.frexp(lo)[1].double() - 8))
-        at_power = (torch.frexp(lo)[0].abs() == 0.5) & (lo > 0)
-        lo = torch.where(lo > least, lo - torch.where(at_power, gap / 2, gap), lo)
+        least = torch.minimum(part.min(-1, keepdim=True)[0], torch.zeros((), dtype=torch.double, device=x.device))
+        most = torch.maximum(part.max(-1, keepdim=True)[0], torch.zeros((), dtype=torch.double, device=x.device))
         # (a step is a held number: float32's subtraction and division, then float16's rounding)
-        way = (most.float() - lo.float()).div(torch.full_like(most, 15.0, dtype=torch.float32))
+        way = (most.float() - least.float()).div(torch.full_like(most, 15.0, dtype=torch.float32))
         step = way.clamp(max=65504.0).half().double()
-        code = torch.where(step > 0, ((part - lo) / torch.where(step > 0, step, 1.0)).round(), 0.0)
-        out[..., a:a + GROUP] = lo + step * code.clamp(0, 15)
+        by = torch.where(step > 0, step, 1.0)
+        zero = (-least / by).round().clamp(max=15.0)
+        whole = ((part / by).round() + zero).clamp(0, 15) - zero
+        out[..., a:a + GROUP] = step * whole
     return out
 
 
