@@ -50,6 +50,8 @@ def parse_args(argv=None):
                     help="with --model-dir, bfloat16: round 32-bit matrices to bfloat16")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--num-pages", type=int, default=-1)
+    ap.add_argument("--kv-bits", type=int, default=None, choices=[4],
+                    help="hold keys and values in 4 bits (default: in --dtype)")
     ap.add_argument("--layers", type=int, default=None, help="fewer layers (random weights only)")
     ap.add_argument("--decode-ahead", type=_bool, default=True,
                     help="launch decode steps before the last one's tokens are read")
@@ -99,7 +101,7 @@ def main(args) -> None:
         max_num_batched_tokens=args.max_num_batched_tokens, max_num_seqs=args.max_num_seqs,
         chunked_prefill=args.chunked_prefill, eos=-1, dtype=model.ctx.dtype,
         kvcache_block_size=args.page_size, num_kvcache_blocks=args.num_pages,
-        decode_ahead=args.decode_ahead))
+        kv_bits=args.kv_bits, decode_ahead=args.decode_ahead))
     params = [SamplingParams(temperature=0.6, ignore_eos=True, max_tokens=n) for n in output_lens]
     llm.generate([[1, 2, 3]], SamplingParams(max_tokens=8, ignore_eos=True), use_tqdm=False)
     torch.cuda.synchronize()

@@ -52,6 +52,8 @@ def parse_args(argv=None):
                          "bfloat16 (default: they stay 32-bit, on the float32 kernels)")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--num-pages", type=int, default=-1)
+    ap.add_argument("--kv-bits", type=int, default=None, choices=[4],
+                    help="hold keys and values in 4 bits (default: in --dtype)")
     ap.add_argument("--max-num-batched-tokens", type=int, default=16384)
     ap.add_argument("--max-num-seqs", type=int, default=512)
     ap.add_argument("--max-model-len", type=int, default=None)
@@ -110,6 +112,7 @@ def main(args) -> None:
         max_model_len=args.max_model_len or min(int(spec.max_position), 40960),
         eos=eos, dtype=dtype, enforce_eager=args.enforce_eager,
         kvcache_block_size=args.page_size, num_kvcache_blocks=args.num_pages,
+        kv_bits=args.kv_bits,
         max_num_batched_tokens=args.max_num_batched_tokens, max_num_seqs=args.max_num_seqs,
         chunked_prefill=args.chunked_prefill, seed=args.seed,
         enable_prefix_caching=args.prefix_caching)

@@ -7,6 +7,8 @@ page, [runs, num_pages, nkv, hd, P].  One key/value head's part of a page is con
 in both; keys are contiguous along the head size (the reduction of q.k) and values along
 the positions (the reduction of p.v), which is what the matrix-core kernels read without
 a transpose.  A run's view is `LayerCache`.
+With `kv_bits` 4 both are uint8 [runs, num_pages, nkv, P / 16, bytes of a block]
+(cache/packed.py); latent vectors and states keep their types.
 A group of latent runs (one vector per token that all heads share) has one tensor
 [runs, num_pages, P, dim] and no second one.
 Per-request state of fixed size lives in [num_slots + 1, *shape] tensors, one per run
@@ -20,6 +22,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from tokensprint_amd.cache.packed import packed_block_bytes, packed_pages_shape
 from tokensprint_amd.cache.pages import GroupLayout
 from tokensprint_amd.parts.base import PagedKVNeed, PagedLatentNeed, SlotStateNeed, flat_needs
 
@@ -45,11 +48,14 @@ def group_runs(needs) -> tuple[list[GroupLayout], dict[int, int]]:
     return groups, group_of_run
 
 
-def page_bytes(groups: list[GroupLayout], page_size: int, dtype: torch.dtype) -> int:
+def page_bytes(groups: list[GroupLayout], page_size: int, dtype: torch.dtype,
+               kv_bits: int | None = None) -> int:
     """Bytes one page id costs summed over all groups (each group has its own pool)."""
     item = torch.empty((), dtype=dtype).element_size()
-    return sum(len(g.runs) * (1 if g.kind == "latent" else 2) * g.num_kv_heads * page_size
-               * g.head_dim * item for g in groups)
+    packed = [g for g in groups if g.kind != "latent"] if kv_bits is not None else []
+    return sum(len(g.runs) * 2 * g.num_kv_heads * (page_size // 16) * packed_block_bytes(g.head_dim)
+               for g in packed) + sum(len(g.runs) * (1 if g.kind == "latent" else 2) * g.num_kv_heads * page_size
+               * g.head_dim * item for g in groups if g not in packed)
 
 
 def state_bytes(needs, num_slots: int) -> int:
@@ -73,15 +79,19 @@ class LayerCache:
     group: int                     # index into the batch's block tables
     page_size: int
     num_pages: int
-    k_pages: torch.Tensor | None   # [num_pages, nkv, P, hd]; a latent run's [num_pages, P, dim]
-    v_pages: torch.Tensor | None   # [num_pages, nkv, hd, P]; None for a latent run
+    k_pages: torch.Tensor | None   # [num_pages, nkv, P, hd]; a latent run's [num_pages, P, dim];
+                                   # 4 bits: uint8 [num_pages, nkv, P / 16, bytes]
+    v_pages: torch.Tensor | None   # [num_pages, nkv, hd, P] (4 bits: as k_pages); None for a latent run
     state: torch.Tensor | None = None   # [num_slots + 1, *shape]: the first fixed-size state
     states: dict = field(default_factory=dict)   # every fixed-size state of the run, by name
 
 
 class CacheStorage:
     def __init__(self, needs, page_size: int, num_pages, num_slots: int,
-                 dtype: torch.dtype, device) -> None:
+                 dtype: torch.dtype, device, kv_bits: int | None = None) -> None:
+        if kv_bits not in (None, 4):
+            raise ValueError(f"kv_bits={kv_bits}: keys and values are held in the cache's type "
+                             "(None) or in 4 bits")
         self.groups, group_of_run = group_runs(needs)
         counts = [num_pages] * len(self.groups) if isinstance(num_pages, int) else list(num_pages)
         self.page_size, self.num_pages, self.num_slots = page_size, counts, num_slots
@@ -91,6 +101,11 @@ class CacheStorage:
                 self.k_tensors.append(torch.zeros(
                     len(g.runs), n, page_size, g.head_dim, dtype=dtype, device=device))
                 self.v_tensors.append(None)
+                continue
+            if kv_bits is not None:
+                shape = (len(g.runs), *packed_pages_shape(n, g.num_kv_heads, page_size, g.head_dim))
+                for tensors in (self.k_tensors, self.v_tensors):
+                    tensors.append(torch.zeros(shape, dtype=torch.uint8, device=device))
                 continue
             self.k_tensors.append(torch.zeros(
                 len(g.runs), n, g.num_kv_heads, page_size, g.head_dim, dtype=dtype, device=device))

@@ -51,6 +51,7 @@ class Config:
     decode_ahead: bool = True             # launch a decode step before the last one's tokens are read
     fold_merge: bool = True               # a decode step's attention merges its key splits itself
                                           # (False: a merge kernel of its own after it)
+    kv_bits: int | None = None            # 4: keys and values held in 4 bits (None: in `dtype`)
 
     def __post_init__(self) -> None:
         if not os.path.isdir(self.model):
@@ -62,5 +63,11 @@ class Config:
                              "max_model_len >= 2")
         if self.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"dtype must be torch.bfloat16 or torch.float32, got {self.dtype}")
+        if self.kv_bits not in (None, 4):
+            raise ValueError(f"kv_bits must be None or 4, got {self.kv_bits}")
+        if self.kv_bits is not None and (self.kvcache_block_size < 16 or
+                                         self.kvcache_block_size & (self.kvcache_block_size - 1)):
+            raise ValueError("kv_bits=4 needs a kvcache_block_size that is a power of two from 16, "
+                             f"got {self.kvcache_block_size}")
         if not 0.0 < self.gpu_memory_utilization <= 1.0:
             raise ValueError("gpu_memory_utilization must be in (0, 1]")

@@ -1,0 +1,6 @@
+// Attention over keys and values of 4 bits: float32 activations, scores with a cap, a distance bias or a query temperature.
+#include "packed_attention_kernel.h"
+
+int launch_packed_f32_scores(const PackedArgs& args, bool coop, hipStream_t stream) {
+  TS_PACKED_CASES(3, true, float);
+}

@@ -65,7 +65,7 @@ class LLMEngine:
             config.num_kvcache_blocks = num_pages
         self.runner = ModelRunner(
             model, page_size=page, num_pages=num_pages, num_slots=config.max_num_seqs,
-            graph_max_len=graph_len)
+            graph_max_len=graph_len, kv_bits=config.kv_bits)
         if config.enable_prefix_caching:
             self.runner.manager.enable_prefix_cache()
         if config.warmup and on_gpu:
@@ -117,7 +117,8 @@ class LLMEngine:
         torch.cuda.synchronize(device)
         torch.cuda.empty_cache()
         probe = ModelRunner(model, page_size=page, num_pages=-(-tokens // page) + requests,
-                            num_slots=config.max_num_seqs, graph_max_len=graph_len)
+                            num_slots=config.max_num_seqs, graph_max_len=graph_len,
+                            kv_bits=config.kv_bits)
         torch.cuda.synchronize(device)
         before = torch.cuda.memory_reserved(device)
         torch.cuda.reset_peak_memory_stats(device)
@@ -151,7 +152,7 @@ class LLMEngine:
         states = state_bytes(model.cache_needs(), config.max_num_seqs)
         available = free * config.gpu_memory_utilization - steps - states
         pages = ModelRunner.pages_that_fit(model, config.kvcache_block_size, int(available),
-                                           config.dtype)
+                                           config.dtype, config.kv_bits)
         # no request can use more than max_model_len tokens
         cap = config.max_num_seqs * (-(-config.max_model_len // config.kvcache_block_size) + 1)
         pages = min(pages, cap)

@@ -21,15 +21,16 @@ from tokensprint_amd.models.model import Model
 class ModelRunner:
     def __init__(self, model: Model, *, page_size: int, num_pages: int, num_slots: int,
                  cache_dtype: torch.dtype | None = None, graph_max_len: int | None = None,
-                 graph_max_batch: int = 256) -> None:
+                 graph_max_batch: int = 256, kv_bits: int | None = None) -> None:
         """`graph_max_len`: the longest request a captured decode graph must serve (its
-        block tables are that wide); None means every step runs eagerly."""
+        block tables are that wide); None means every step runs eagerly.  `kv_bits` 4: keys
+        and values are held in 4 bits."""
         self.model = model
         self.device = model.ctx.device
         self.dtype = model.ctx.dtype
         needs = model.cache_needs()
         self.storage = CacheStorage(needs, page_size, num_pages, num_slots,
-                                    cache_dtype or self.dtype, self.device)
+                                    cache_dtype or self.dtype, self.device, kv_bits)
         self.manager = CacheManager(self.storage.groups, page_size, num_pages, num_slots,
                                     state_runs=self.storage.state_runs)
         self.builder = BatchBuilder(self.device, len(self.storage.groups),
@@ -55,12 +56,12 @@ class ModelRunner:
 
     @staticmethod
     def pages_that_fit(model: Model, page_size: int, free_bytes: int,
-                       cache_dtype: torch.dtype) -> int:
+                       cache_dtype: torch.dtype, kv_bits: int | None = None) -> int:
         """Page ids affordable in `free_bytes` (every group gets that many pages);
         the arithmetic of engine/generation/model_runner.py:400-411."""
         from tokensprint_amd.cache.storage import group_runs
         groups, _ = group_runs(model.cache_needs())
-        per_page = page_bytes(groups, page_size, cache_dtype)
+        per_page = page_bytes(groups, page_size, cache_dtype, kv_bits)
         return int(free_bytes // max(per_page, 1))
 
     def build(self, entries: list[StepEntry], table_width=None) -> StepBatch:

@@ -151,6 +151,12 @@ class Dispatch:
     cooperative_workgroups: int = 512
     per_wave_workgroups: int = 4096
 
+    # ---- attention over keys and values of 4 bits: up to so many tiles of 16 rows (times key/value
+    # heads) a workgroup per tile and share of its keys, above it a wavefront per tile; the
+    # workgroups that shares are made for.
+    packed_items: int = 2048
+    packed_workgroups: int = 1024
+
     # ---- recurrences.  A step whose longest portion has more tokens than this runs in chunks of
     # 64 tokens as products of matrices, below it every entry is walked whole by one launch.
     # Three launches have a length of their own, a walked token costs 0.24 to 0.28 us (16 heads

@@ -14,6 +14,7 @@ from ctypes import Structure, byref, c_float, c_int, c_int64, c_void_p
 import numpy as np
 import torch
 
+from tokensprint_amd.cache.packed import packed_pages_shape
 from tokensprint_amd.kernels.build import build, find_library
 from tokensprint_amd.kernels.dispatch import default_dispatch
 from tokensprint_amd.kernels.stream import NormedPair, PreparedRows, UnmergedRows
@@ -71,6 +72,14 @@ class AttentionDecodeArgs(Structure):
     ]
 
 
+class PackedArgs(Structure):
+    _fields_ = [
+        ("base", AttentionArgs), ("tiles", c_void_p), ("partial_o", c_void_p),
+        ("partial_ml", c_void_p), ("arrivals", c_void_p), ("num_tiles", c_int),
+        ("rows_per_token", c_int), ("head_blocks", c_int), ("num_splits", c_int), ("span", c_int),
+    ]
+
+
 class PromptStream(Structure):
     _fields_ = [
         ("rows", c_void_p), ("sumsq", c_void_p), ("resid", c_void_p), ("norm_w", c_void_p),
@@ -93,6 +102,7 @@ def _load_library() -> ctypes.CDLL:
     lib = ctypes.CDLL(str(path))
     lib.ts_last_error.restype = ctypes.c_char_p
     lib.ts_chunked_scratch.restype = c_int64
+    lib.ts_capture_id.restype = c_int64
     if lib.ts_abi_version() != ABI_VERSION:
         raise KernelError(f"{path} has interface version {lib.ts_abi_version()}, "
                           f"this package needs {ABI_VERSION}")
@@ -154,6 +164,9 @@ class HipOps:
         # `fold_merge = False` gives the merge a kernel of its own again.
         self.fold_merge = True
         self._arrivals = torch.zeros(4096, dtype=torch.int32, device=self.device)
+        # the same for attention over a cache of 4 bits, an array for each stream and for each
+        # capture (see _counts)
+        self._count_arrays = {}
 
     # ------------------------------------------------------------ helpers
     def _stream(self):
@@ -177,6 +190,22 @@ class HipOps:
         of the decode kernel's own merge at zero.  Called after a failed call, and by the
         engine before its warm-up step and before graphs are captured."""
         self._arrivals.zero_()
+        if self._raw_stream(self._device_index) == 0 or not torch.cuda.is_current_stream_capturing():
+            for counts in self._count_arrays.values():
+                counts.zero_()
+
+    def _counts(self, n):
+        """At least `n` zeros in which workgroups count themselves in, left as zeros by every
+        launch.  Launches of one stream may share an array, one after the other; two
+        streams have each their own, and so has each capture, whose graph may be replayed on
+        any stream beside any other (its zeros are made in the graph)."""
+        stream = self._raw_stream(self._device_index)
+        key = stream, self.lib.ts_capture_id(c_void_p(stream)) if stream else 0
+        counts = self._count_arrays.get(key)
+        if counts is None or counts.numel() < n:
+            counts = torch.zeros(max(n, 4096), dtype=torch.int32, device=self.device)
+            self._count_arrays[key] = counts
+        return counts
 
     def _check(self, name, t, dtype=None, shape=None, ndim=None):
         # (written for the case that all is well, which is every call of a working engine:
@@ -902,10 +931,15 @@ class HipOps:
 
     def _check_cache(self, cache, table, batch, nkv, head_dim):
         P = cache.page_size
-        self._check("k_pages", cache.k_pages, self._FLOATS,
-                    shape=(cache.num_pages, nkv, P, head_dim))
-        self._check("v_pages", cache.v_pages, cache.k_pages.dtype,
-                    shape=(cache.num_pages, nkv, head_dim, P))
+        if cache.k_pages.dtype is torch.uint8:       # keys and values in 4 bits
+            shape = packed_pages_shape(cache.num_pages, nkv, P, head_dim)
+            self._check("k_pages", cache.k_pages, torch.uint8, shape=shape)
+            self._check("v_pages", cache.v_pages, torch.uint8, shape=shape)
+        else:
+            self._check("k_pages", cache.k_pages, self._FLOATS,
+                        shape=(cache.num_pages, nkv, P, head_dim))
+            self._check("v_pages", cache.v_pages, cache.k_pages.dtype,
+                        shape=(cache.num_pages, nkv, head_dim, P))
         self._check("block table", table, torch.int32, ndim=2)
         if table.shape[0] != batch.num_entries:
             raise ValueError("block table rows differ from the batch's entries")
@@ -929,6 +963,9 @@ class HipOps:
             a.k_dst, a.v_dst = cache.k_pages.data_ptr(), cache.v_pages.data_ptr()
             a.table, a.table_width = table.data_ptr(), table.shape[1]
             a.page_size, a.paged, a.store_kv = cache.page_size, 1, 1
+            if cache.k_pages.dtype is torch.uint8:
+                self._call(self.lib.ts_pack_prepare, byref(a), cache_type, self._stream())
+                return q
             cache_type = _TYPE_CODE[cache.k_pages.dtype]
         self._call(self.lib.ts_qk_prepare, byref(a), _TYPE_CODE[qkv.dtype], cache_type,
                    self._stream())
@@ -972,10 +1009,36 @@ class HipOps:
         T, nkv, hd = k.shape
         self._check_cache(cache, table, batch, nkv, hd)
         self._check("positions", batch.positions, torch.int32, shape=(T,))
+        if cache.k_pages.dtype is torch.uint8:
+            self._check("entry_of_token", batch.entry_of_token, torch.int32, shape=(T,))
+            self._call(self.lib.ts_pack_store, _ptr(k), _ptr(v), _TYPE_CODE[k.dtype],
+                       _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(batch.positions),
+                       _ptr(batch.entry_of_token), _ptr(table), table.shape[1], T, nkv, hd,
+                       cache.page_size, self._stream())
+            return
         self._call(self.lib.ts_kv_store, _ptr(k), _ptr(v), _TYPE_CODE[k.dtype],
                    _ptr(cache.k_pages), _ptr(cache.v_pages), _TYPE_CODE[cache.k_pages.dtype],
                    _ptr(batch.positions), _ptr(batch.entry_of_token), _ptr(table),
                    table.shape[1], T, nkv, hd, cache.page_size, self._stream())
+
+    def kv_values(self, batch, table, cache, *, num_kv_heads, head_dim, out_dtype):
+        """The keys and values that a cache of 4 bits holds for the batch's tokens, two tensors
+        [T, num_kv_heads, head_dim]; tokens without a page read as zeros."""
+        if cache.k_pages.dtype is not torch.uint8:
+            raise TypeError(f"kv_values reads a cache of 4 bits; this one holds {cache.k_pages.dtype}")
+        if out_dtype not in _TYPE_CODE:
+            raise TypeError(f"kv_values: out_dtype {out_dtype}, expected one of {self._FLOATS}")
+        T = batch.num_tokens
+        self._check_cache(cache, table, batch, num_kv_heads, head_dim)
+        self._check("positions", batch.positions, torch.int32, shape=(T,))
+        self._check("entry_of_token", batch.entry_of_token, torch.int32, shape=(T,))
+        k = torch.empty(T, num_kv_heads, head_dim, dtype=out_dtype, device=self.device)
+        v = torch.empty_like(k)
+        self._call(self.lib.ts_pack_values, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(k),
+                   _ptr(v), _TYPE_CODE[out_dtype], _ptr(batch.positions),
+                   _ptr(batch.entry_of_token), _ptr(table), table.shape[1], T, num_kv_heads,
+                   head_dim, cache.page_size, self._stream())
+        return k, v
 
     # ------------------------------------------------------------ attention
     def paged_attention(self, q, batch, table, cache, *, num_heads, num_kv_heads, head_dim,
@@ -1000,7 +1063,9 @@ class HipOps:
                                   head_dim, scale, window, sink, chunk, softcap, slopes, q_temp,
                                   keep_first)
         extras = softcap is not None or slopes is not None or q_temp is not None
-        if (q.dtype == torch.bfloat16 and cache.k_pages.dtype == torch.bfloat16
+        if cache.k_pages.dtype is torch.uint8:
+            self._attention_packed(a, batch, num_heads // num_kv_heads, q.dtype)
+        elif (q.dtype == torch.bfloat16 and cache.k_pages.dtype == torch.bfloat16
                 and head_dim % 16 == 0 and head_dim <= 256 and cache.page_size % 4 == 0):
             # (scores with extras: of the kernels for long portions those for pages of a power
             # of two know them)
@@ -1031,6 +1096,40 @@ class HipOps:
             self._call(self.lib.ts_attention_generic, byref(a), _TYPE_CODE[q.dtype],
                        _TYPE_CODE[cache.k_pages.dtype], self._stream())
         return out
+
+    def _attention_packed(self, a, batch, group, dtype):
+        """Attention over a cache of 4 bits: tiles of 16 rows (query heads of a key/value head x
+        tokens); few tiles have a workgroup each and share of their keys, many a wavefront
+        each."""
+        if not a.scale > 0:
+            raise ValueError(f"attention over keys of 4 bits: scale={a.scale} must be positive")
+        m = PackedArgs()
+        m.base = a
+        m.rows_per_token, m.head_blocks = min(group, 16), -(-group // 16)
+        if batch.max_q_len == 1:
+            m.num_tiles = batch.num_entries
+        else:
+            tiles, m.num_tiles = self._attention_tiles(batch, 16 // m.rows_per_token)
+            m.tiles = tiles.data_ptr()
+        items = m.num_tiles * a.nkv * m.head_blocks
+        reach = self._reach(a)
+        keys = batch.max_ctx_len if reach == 0 else min(batch.max_ctx_len, reach + batch.max_q_len + 64)
+        d = self.dispatch
+        coop = items <= d.packed_items
+        if coop:
+            # shares of the keys: as long as `packed_workgroups` workgroups leave them, of the
+            # longest context's
+            chunks = -(-keys // 128)
+            m.span = 128 * max(1, -(-chunks * items // d.packed_workgroups),
+                               -(-chunks // 256))
+            m.num_splits = -(-keys // m.span)
+            if m.num_splits > 1:
+                hd = -(-a.hd // 32) * 32
+                po = torch.empty(items * m.num_splits * 16 * hd, dtype=torch.float32, device=self.device)
+                pml = torch.empty(items * m.num_splits * 16 * 2, dtype=torch.float32, device=self.device)
+                m.partial_o, m.partial_ml = po.data_ptr(), pml.data_ptr()
+                m.arrivals = self._counts(items).data_ptr()
+        self._call(self.lib.ts_packed_attention, byref(m), _TYPE_CODE[dtype], int(coop), self._stream())
 
     def attend(self, qkv, batch, table, cache, write_cache, *, num_heads, num_kv_heads,
                kv_in_row, head_dim, q_weight, k_weight, eps, cos_sin, scale, window,
