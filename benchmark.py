@@ -50,6 +50,9 @@ def parse_args(argv=None):
                     help="with --model-dir, bfloat16: round 32-bit matrices to bfloat16")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--num-pages", type=int, default=-1)
+    ap.add_argument("--weight-bits", type=int, default=None, choices=[8],
+                    help="hold attention's projections and dense feed-forwards in 8 bits and run "
+                         "their products in 8-bit numbers")
     ap.add_argument("--kv-bits", type=int, default=None, choices=[4],
                     help="hold keys and values in 4 bits (default: in --dtype)")
     ap.add_argument("--layers", type=int, default=None, help="fewer layers (random weights only)")
@@ -81,14 +84,15 @@ def main(args) -> None:
     seed(0)
     prompts, output_lens = make_workload(args)
     if args.model_dir is not None:
-        _, model = load_model(args.model_dir, args.dtype, "cuda:0", cast_32bit=args.cast_weights)
+        _, model = load_model(args.model_dir, args.dtype, "cuda:0", cast_32bit=args.cast_weights,
+                              weight_bits=args.weight_bits)
         model_dir = str(args.model_dir)
     else:
         raw = json.loads(args.config_json.read_text()) if args.config_json is not None \
             else load_named_config(args.model_name)
         if args.layers:
             raw["num_hidden_layers"] = args.layers
-        _, model = random_model(raw, 0, args.dtype, "cuda:0")
+        _, model = random_model(raw, 0, args.dtype, "cuda:0", weight_bits=args.weight_bits)
         model_dir = tempfile.gettempdir()
     spec = model.spec
     max_model_len = args.max_model_len or min(int(spec.max_position), 40960)

@@ -52,6 +52,9 @@ def parse_args(argv=None):
                          "bfloat16 (default: they stay 32-bit, on the float32 kernels)")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--num-pages", type=int, default=-1)
+    ap.add_argument("--weight-bits", type=int, default=None, choices=[8],
+                    help="hold attention's projections and dense feed-forwards in 8 bits and run "
+                         "their products in 8-bit numbers")
     ap.add_argument("--kv-bits", type=int, default=None, choices=[4],
                     help="hold keys and values in 4 bits (default: in --dtype)")
     ap.add_argument("--max-num-batched-tokens", type=int, default=16384)
@@ -87,7 +90,8 @@ def main(args) -> None:
         raise ValueError("--config-json describes random weights: give --random-weights SEED")
     elif model_dir is None:
         model_dir = args.cache_dir / get_model_repo_id(args.model_name).split("/")[-1]
-    _, model = load_model(model_dir, dtype, "cuda:0", cast_32bit=args.cast_weights)
+    _, model = load_model(model_dir, dtype, "cuda:0", cast_32bit=args.cast_weights,
+                          weight_bits=args.weight_bits)
     spec = model.spec           # sizes and the end-of-sequence token come from the model as
                                 # built, whatever architecture config.json named
 

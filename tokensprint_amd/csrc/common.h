@@ -187,6 +187,17 @@ __device__ __forceinline__ float gated_unit(float gate, float up, float limit) {
   return gate / (1.f + expf(-gate)) * up;
 }
 
+// The whole number nearest to x / step (inv: about 1 / step), ties to even: the estimate is at most
+// one off, and what is left of x is exact in float32 wherever the estimate is small.
+__device__ __forceinline__ float nearest_whole(float x, float step, float inv) {
+  float c = rintf(x * inv);
+  const float left = fmaf(-c, step, x), half = 0.5f * step;
+  const bool odd = ((int)c & 1) != 0;
+  if (left > half || (left == half && odd)) c += 1.f;
+  else if (left < -half || (left == -half && odd)) c -= 1.f;
+  return c;
+}
+
 // Dispatch a two-way element type code to a template argument.
 #define TS_DISPATCH_TYPE(code, T, ...)                    \
   if ((code) == TS_F32) { typedef float T; __VA_ARGS__; } \

@@ -34,12 +34,14 @@
 // its BM rows before it sends for its first operands.  HEADS is SCALED for a q/k/v projection with
 // heads of as many elements as a tile has columns: the tile, rounded, passes LDS and leaves as
 // qk_prepare.hip would have left it (normed and turned queries, keys and values in their pages).
+// INT8: operands of 8-bit whole numbers with a scale for each row of both (gemm_int8.h).  A step's slabs are
+// 128 bytes of every row as ever, so everything but the instruction and the epilogue is as for bfloat16; `K` counts pairs of bytes.
 #pragma once
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
 
-#include "gemm_common.h"
+#include "gemm_int8.h"
 #include "qk_prepare.h"
 
 namespace {
@@ -70,7 +72,11 @@ struct TiledHeadsArgs : TiledArgs {
   QkPrepareArgs heads;
 };
 
-constexpr int kPlain = 0, kScaled = 1, kTail = 2, kHeads = 3;
+struct TiledInt8Args : TiledArgs {
+  const float *a_scale, *w_scale;     // [M], [N] (PAIR: [2 N])
+};
+
+constexpr int kPlain = 0, kScaled = 1, kTail = 2, kHeads = 3, kInt8 = 4;
 constexpr int kSliceColumns = 32;   // columns per slice of a row's sum of squares (TAIL)
 
 // One 16-byte piece per lane from global memory (uniform base + per-lane byte offset)
@@ -203,7 +209,14 @@ __device__ __forceinline__ void heads_out(const TiledHeadsArgs& g, int head, int
 }
 
 template <int FORM>
-using TiledArgsOf = std::conditional_t<FORM == kHeads, TiledHeadsArgs, TiledArgs>;
+using TiledArgsOf = std::conditional_t<FORM == kHeads, TiledHeadsArgs, std::conditional_t<FORM == kInt8, TiledInt8Args, TiledArgs>>;
+
+__device__ __forceinline__ f32x4 tiled_product(bf16x8 w, bf16x8 a, f32x4 acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, a, acc, 0, 0, 0);
+}
+__device__ __forceinline__ i32x4 tiled_product(bf16x8 w, bf16x8 a, i32x4 acc) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, a), acc, 0, 0, 0);
+}
 
 template <int BM, int BN, int GM, int GN, int STAGES, bool PAIR, typename TO, int FORM = kPlain>
 __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf<FORM> g) {
@@ -351,11 +364,12 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
     else dma16((const char*)g.w + (int64_t)kt * 128, off_w[i - LA], dst + BM * 128 + (i - LA) * NW * 1024);
   };
 
-  f32x4 acc[TN][TM];
+  typedef std::conditional_t<FORM == kInt8, i32x4, f32x4> Sums;
+  Sums acc[TN][TM];
 #pragma unroll
   for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
-    for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = Sums{0, 0, 0, 0};
 
   // a lane's reads: row r of a 16-row block, the piece that holds k = 32 ks + 8 gq ..
   const int swz = (r >> 1) & 7;
@@ -382,7 +396,7 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
     for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
       for (int tm = 0; tm < TM; ++tm) {
-        acc[tn][tm] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.w[tn], f.a[tm], acc[tn][tm], 0, 0, 0);
+        acc[tn][tm] = tiled_product(f.w[tn], f.a[tm], acc[tn][tm]);
         const int idx = tn * TM + tm;
         if constexpr (load) {
           if (idx % EVERY == 0 && idx / EVERY < LOADS) issue_one(stage, kt, idx / EVERY);
@@ -467,8 +481,7 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
         const int half = b / (2 * H), ks = b / H % 2, t = b % H;
 #pragma unroll
         for (int tn = 0; tn < TN; ++tn)
-          acc[tn][half * H + t] =
-              __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[ks][tn], fa[t], acc[tn][half * H + t], 0, 0, 0);
+          acc[tn][half * H + t] = tiled_product(fw[ks][tn], fa[t], acc[tn][half * H + t]);
         // the lower half of this step has arrived; its W and upper half have been read
         if (b == H) meet(std::integral_constant<int, behind >= 1 ? LOADS : 0>{});
         if constexpr (behind >= 1) {
@@ -628,6 +641,41 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
     });
     return;
   }
+  if constexpr (FORM == kInt8) {
+    constexpr int COLS = PAIR ? TN / 2 : TN;
+    auto scales = [&](const float* p, int n) {
+      f32x4 s;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] = p[min(n + e, g.N - 1)];
+      return s;
+    };
+#pragma unroll
+    for (int tn = 0; tn < COLS; ++tn) {
+      const int n = tile_n * (PAIR ? BN / 2 : BN) + wn * (PAIR ? WN / 2 : WN) + tn * 16 + gq * 4;
+      if (n >= g.N) continue;
+      const f32x4 s0 = scales(g.w_scale, n);
+      f32x4 s1;
+      if constexpr (PAIR) s1 = scales(g.w_scale + g.N, n);
+#pragma unroll
+      for (int tm = 0; tm < TM; ++tm) {
+        const int m = m0 + wm * WM + tm * 16 + r;
+        if (m >= g.M) continue;
+        const float row = g.a_scale[m];
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = (float)acc[tn][tm][e] * s0[e] * row;
+          if constexpr (PAIR) {
+            const float up = (float)acc[tn + TN / 2][tm][e] * s1[e] * row;
+            const float gc = fminf(v[e], top), uc = fminf(fmaxf(up, -top), top) + lift;
+            v[e] = gc * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(gc * fmaf(cubic, gc * gc, slope))) * uc;
+          }
+        }
+        store4<TO>(c + (int64_t)m * g.N + n, v, g.N - n);
+      }
+    }
+    return;
+  } else {
 #pragma unroll
   for (int tm = 0; tm < TM; ++tm) {
     const int m = m0 + wm * WM + tm * 16 + r;
@@ -661,6 +709,7 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
         store4<TO>(c + (int64_t)m * g.N + n, acc[tn][tm], g.N - n);
       }
     }
+  }
   }
 }
 
@@ -744,7 +793,7 @@ inline int cheapest_tile(const TiledArgs& g, bool pair, int least_rows = 0) {
 }
 
 template <bool PAIR, typename TO, int FORM = kPlain>
-int choose_tile(const TiledArgs& g, int tile, hipStream_t stream) {
+int choose_tile(const TiledArgsOf<FORM>& g, int tile, hipStream_t stream) {
   if (tile == 0) tile = cheapest_tile(g, PAIR);
   switch (tile) {
     case 1: return launch_tiled<256, 128, 4, 2, 3, PAIR, TO, FORM>(g, stream);

@@ -55,17 +55,6 @@ __device__ __forceinline__ int64_t pack_block(int page, int nkv, int kvh, int pa
   return (((int64_t)page * nkv + kvh) * (page_size / kPackTokens) + slot / kPackTokens) * bytes;
 }
 
-// The whole number nearest to x / step (inv: about 1 / step), ties to even: the estimate is at most
-// one off, and what is left of x is exact in float32 wherever the estimate is small.
-__device__ __forceinline__ float pack_round(float x, float step, float inv) {
-  float c = rintf(x * inv);
-  const float left = fmaf(-c, step, x), half = 0.5f * step;
-  const bool odd = ((int)c & 1) != 0;
-  if (left > half || (left == half && odd)) c += 1.f;
-  else if (left < -half || (left == -half && odd)) c -= 1.f;
-  return c;
-}
-
 struct PackGroup {
   _Float16 step;
   float zero;
@@ -90,10 +79,10 @@ __device__ __forceinline__ PackGroup pack_eight(float (&v)[8], unsigned (&code)[
   PackGroup p;
   p.step = (_Float16)fminf((hi - lo) / 15.f, 65504.f);
   const float step = (float)p.step, inv = step > 0.f ? 1.f / step : 0.f;
-  p.zero = step > 0.f ? fminf(pack_round(-lo, step, inv), 15.f) : 0.f;
+  p.zero = step > 0.f ? fminf(nearest_whole(-lo, step, inv), 15.f) : 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    code[j] = step > 0.f ? (unsigned)fminf(fmaxf(pack_round(v[j], step, inv) + p.zero, 0.f), 15.f) : 0u;
+    code[j] = step > 0.f ? (unsigned)fminf(fmaxf(nearest_whole(v[j], step, inv) + p.zero, 0.f), 15.f) : 0u;
   return p;
 }
 

@@ -45,21 +45,29 @@ def build_model(raw_config: dict, dtype, device, ops=None):
     return config, Model(spec, ctx)
 
 
-def load_model(model_dir, dtype="bfloat16", device="cuda:0", ops=None, cast_32bit=False):
+def load_model(model_dir, dtype="bfloat16", device="cuda:0", ops=None, cast_32bit=False,
+               weight_bits=None):
     """(typed config, Model with weights) from a folder with config.json and safetensors.
     `cast_32bit`: in a bfloat16 run, round matrices the files store in 32-bit to bfloat16
-    (by default they stay 32-bit and are served by the float32 kernels)."""
+    (by default they stay 32-bit and are served by the float32 kernels).  `weight_bits` 8:
+    hold attention's projections and dense feed-forwards in 8 bits, with a scale per output
+    channel, and run their products in 8-bit numbers (rows with a scale each)."""
     config, model = build_model(read_config_json(model_dir), dtype, device, ops)
     load_weights(model, model_dir, model.ctx.dtype, model.ctx.device, cast_32bit=cast_32bit)
+    if weight_bits is not None:
+        model.quantize_weights(weight_bits)
     return config, model
 
 
 def random_model(raw_config: dict, seed: int, dtype="bfloat16", device="cuda:0", ops=None,
-                 std: float = 0.02):
-    """A model with random weights made directly in memory (no folder is written)."""
+                 std: float = 0.02, weight_bits=None):
+    """A model with random weights made directly in memory (no folder is written);
+    `weight_bits` as in `load_model`."""
     from tokensprint_amd.weights.random_init import random_tensors
     config, model = build_model(raw_config, dtype, device, ops)
     tensors = random_tensors(raw_config, seed, dtype=model.ctx.dtype, std=std,
                              device=model.ctx.device)
     load_weights(model, TensorDict(tensors), model.ctx.dtype, model.ctx.device)
+    if weight_bits is not None:
+        model.quantize_weights(weight_bits)
     return config, model

@@ -17,6 +17,7 @@ import torch
 from tokensprint_amd.cache.packed import packed_pages_shape
 from tokensprint_amd.kernels.build import build, find_library
 from tokensprint_amd.kernels.dispatch import default_dispatch
+from tokensprint_amd.kernels.int8 import Int8Rows, Int8Weight, row_bytes
 from tokensprint_amd.kernels.stream import NormedPair, PreparedRows, UnmergedRows
 
 ABI_VERSION = 3
@@ -368,7 +369,10 @@ class HipOps:
 
     # ------------------------------------------------------------ matrix product
     def linear(self, x, weight, out_dtype):
-        """x [M, K] times weight [N, K] transposed -> [M, N] in out_dtype."""
+        """x [M, K] times weight [N, K] transposed -> [M, N] in out_dtype.  With an Int8Weight
+        the product is one of 8-bit numbers: x (or Int8Rows as they are) with a scale per row."""
+        if weight.__class__ is Int8Weight:
+            return self._int8_product(x, weight, out_dtype)
         x = self._rows(x)
         self._check("x", x, self._FLOATS, ndim=2)
         self._check("weight", weight, self._FLOATS, ndim=2)
@@ -830,7 +834,13 @@ class HipOps:
         the product in one kernel where it can be (bfloat16 weights, at most 16 rows);
         otherwise the same from separate kernels.  `delta` may be None.  With `silu_mul`
         the weight is [Wg; Wu] and the result silu(h Wg^T) * (h Wu^T).  The returned
-        residual stream may or may not be the tensor passed in."""
+        residual stream may or may not be the tensor passed in.  With an Int8Weight the normed
+        rows go into the product in 8 bits, and the returned stream is another tensor unless
+        there is nothing to add."""
+        if weight.__class__ is Int8Weight:
+            rows, resid = self.norm_quantize_rows(resid, delta, norm_weight, eps)
+            product = self.linear_silu_mul if silu_mul else self.linear
+            return product(rows, weight, out_dtype), resid
         self._check("resid", resid, torch.float32, ndim=2)
         if isinstance(delta, PreparedRows):     # already added in, by linear_into_stream
             return self._prepared_linear(resid, delta, norm_weight, eps, weight, out_dtype,
@@ -870,7 +880,9 @@ class HipOps:
 
     def linear_silu_mul(self, x, weight, out_dtype, limit=None, act="silu"):
         """silu(x Wg^T) * (x Wu^T) for weight = [Wg; Wu] stacked by rows -> [M, N/2]; `limit`
-        and `act` choose the gated unit as in silu_mul."""
+        and `act` choose the gated unit as in silu_mul.  An Int8Weight as in `linear`."""
+        if weight.__class__ is Int8Weight:
+            return self._int8_product(x, weight, out_dtype, pair=True, unit=self._unit(limit, act))
         x = self._rows(x)
         self._check("x", x, self._FLOATS, ndim=2)
         self._check("weight", weight, self._FLOATS, ndim=2)
@@ -887,6 +899,73 @@ class HipOps:
                        _TYPE_CODE[out_dtype], M, inner, K, 1, self._unit(limit, act), self._stream())
             return out
         return self.silu_mul(self.linear(x, weight, out_dtype), limit, act)
+
+    # ------------------------------------------------------------ products in 8 bits
+    def quantize_rows(self, x):
+        """x [M, K] as Int8Rows: a scale per row, its largest magnitude / 127, and the nearest whole
+        numbers of scales.  A row with an infinity or a NaN gets a scale that is not finite."""
+        x = self._rows(x)
+        self._check("x", x, self._FLOATS, ndim=2)
+        return self._quantized(x, Int8Rows)
+
+    def quantize_weight(self, weight):
+        """A weight [N, K] as an Int8Weight: a scale per output channel."""
+        self._check("weight", weight, self._FLOATS, ndim=2)
+        return self._quantized(weight, Int8Weight)
+
+    def _quantized(self, x, kind):
+        M, K = x.shape
+        row = self._int8_row(K)
+        codes = torch.empty(M, row, dtype=torch.int8, device=self.device)
+        scales = torch.empty(M, dtype=torch.float32, device=self.device)
+        self._call(self.lib.ts_quantize_rows, _ptr(x), _TYPE_CODE[x.dtype], _ptr(codes), _ptr(scales),
+                   M, K, row, self._stream())
+        return kind(codes, scales, K)
+
+    @staticmethod
+    def _int8_row(K):
+        if not 1 <= K <= 131072:
+            raise ValueError(f"rows in 8 bits: {K} elements, 1 to 131,072 are served")
+        return row_bytes(K)
+
+    def norm_quantize_rows(self, resid, delta, norm_weight, eps):
+        """(RMSNorm(resid + delta) as Int8Rows, resid + delta): `delta` may be None, and the returned
+        stream is then `resid` itself, else a new tensor.  The normed rows are quantised in
+        float32, not rounded to another type first."""
+        self._check("resid", resid, torch.float32, ndim=2)
+        M, K = resid.shape
+        self._check("norm weight", norm_weight, torch.float32, shape=(K,))
+        out, row = resid, self._int8_row(K)
+        if delta is not None:
+            delta = self._rows(delta)
+            self._check("delta", delta, self._FLOATS, shape=resid.shape)
+            out = torch.empty_like(resid)
+        codes = torch.empty(M, row, dtype=torch.int8, device=self.device)
+        scales = torch.empty(M, dtype=torch.float32, device=self.device)
+        self._call(self.lib.ts_norm_quantize_rows, _ptr(resid), _ptr(delta),
+                   _TYPE_CODE[delta.dtype] if delta is not None else 0, _ptr(norm_weight),
+                   c_float(eps), _ptr(out if delta is not None else None), _ptr(codes), _ptr(scales),
+                   M, K, row, self._stream())
+        return Int8Rows(codes, scales, K), out
+
+    def _int8_product(self, x, weight, out_dtype, pair=False, unit=None, tile=0):
+        """`tile` as in `gemm_tiled`; 9: the kernel for few rows."""
+        if not isinstance(x, Int8Rows):
+            x = self.quantize_rows(x)
+        if out_dtype not in _TYPE_CODE:
+            raise TypeError(f"a product in 8 bits cannot give {out_dtype}")
+        if x.width != weight.width or (pair and weight.codes.shape[0] % 2):
+            raise ValueError(f"a product in 8 bits: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+        for name, t in (("x", x), ("weight", weight)):
+            rows = t.codes.shape[0]
+            self._check(name + " codes", t.codes, torch.int8, shape=(rows, self._int8_row(t.width)))
+            self._check(name + " scales", t.scales, torch.float32, shape=(rows,))
+        M, N = x.codes.shape[0], weight.codes.shape[0] // 2 if pair else weight.codes.shape[0]
+        out = torch.empty(M, N, dtype=out_dtype, device=self.device)
+        self._call(self.lib.ts_gemm_int8, _ptr(x.codes), _ptr(x.scales), _ptr(weight.codes),
+                   _ptr(weight.scales), _ptr(out), _TYPE_CODE[out_dtype], M, N, x.codes.shape[1],
+                   int(pair), unit or c_float(0.0), tile, self._stream())
+        return out
 
     # ------------------------------------------------------------ q/k preparation
     def _qk_args(self, qkv, batch, *, num_heads, kv_in_row, head_dim, q_weight, k_weight, eps,

@@ -73,6 +73,16 @@ class Model:
             part.load(tensors.get)
         self.enter_tables = {name: tensors[name] for name in self.spec.enter_tables}
 
+    def quantize_weights(self, bits: int) -> None:
+        """The matrices that layers' parts name (attention's projections, dense feed-forwards) in
+        `bits` (8) bits: embedding, output head, norms, recurrences and routed experts stay as
+        they are."""
+        if bits != 8:
+            raise ValueError(f"weights can be held in 8 bits, not in {bits}")
+        for block in self.blocks:
+            for part in block.parts():
+                part.quantize_weights()
+
     # ------------------------------------------------------------ caches
     def cache_needs(self):
         """Per run: the cache need of its block, or None if the run owns no cache.  If the

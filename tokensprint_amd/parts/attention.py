@@ -23,6 +23,8 @@ class GroupedQueryAttention(StreamProducts, Mixer):
     own_kv (False: the layer has no k/v weights and only reads another run's cache).
     """
 
+    eight_bit_weights = ("w_qkv", "w_o")
+
     def __init__(self, params, ctx):
         super().__init__(params, ctx)
         p = params

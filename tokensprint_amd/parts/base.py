@@ -19,6 +19,8 @@ from typing import Any, Callable
 
 import torch
 
+from tokensprint_amd.kernels.int8 import Int8Rows
+
 # ------------------------------------------------------------------ declarations
 
 
@@ -121,7 +123,21 @@ class Part:
             for t in value if isinstance(value, (list, tuple)) else (value,):
                 if isinstance(t, torch.Tensor):
                     out.append(t)
+                elif isinstance(t, Int8Rows):
+                    out += [t.codes, t.scales]
         return out
+
+    #: attributes that hold matrices which go into the provider's `linear`, `norm_linear`,
+    #: `linear_silu_mul` or `last_product` and nowhere else: what a model with weights of 8 bits
+    #: holds so
+    eight_bit_weights: tuple[str, ...] = ()
+
+    def quantize_weights(self) -> None:
+        """Those matrices from the checkpoint's type into 8 bits, a scale per output channel."""
+        for name in self.eight_bit_weights:
+            weight = getattr(self, name)
+            if isinstance(weight, torch.Tensor):
+                setattr(self, name, self.ops.quantize_weight(weight))
 
     def step_read_tensors(self) -> list[torch.Tensor]:
         """The tensors a step reads whole, whatever its tokens are: what a decode step's

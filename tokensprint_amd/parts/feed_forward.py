@@ -23,6 +23,8 @@ class SwiGLU(StreamProducts, FeedForward):
     down; default 'gate_proj.weight', 'up_proj.weight', 'down_proj.weight'), limit (None: the
     plain unit), act ("silu", the default, or "gelu_tanh"), wide_output (the result leaves in float32, for a block that norms it)."""
 
+    eight_bit_weights = ("w_gate_up", "w_down")
+
     def __init__(self, params, ctx):
         super().__init__(params, ctx)
         self.prefix = params["prefix"]
@@ -85,6 +87,8 @@ class PolyNormMLP(FeedForward):
 
     params: prefix, inner_dim, eps."""
 
+    eight_bit_weights = ("w_up", "w_down")
+
     def __init__(self, params, ctx):
         super().__init__(params, ctx)
         self.prefix = params["prefix"]
@@ -112,6 +116,8 @@ class SquaredReluMLP(StreamProducts, FeedForward):
     """down(relu(up(h))^2), no biases; tensors '<prefix>up' and '<prefix>down'.
 
     params: prefix, inner_dim."""
+
+    eight_bit_weights = ("w_up", "w_down")
 
     def __init__(self, params, ctx):
         super().__init__(params, ctx)

@@ -413,6 +413,10 @@ class SideBySide(Mixer):
             self.w_left = (get(self.norms[0]).float() * self.left_scale).contiguous()
             self.w_right = (get(self.norms[1]).float() * self.right_scale).contiguous()
 
+    def quantize_weights(self):
+        self.left.quantize_weights()
+        self.right.quantize_weights()
+
     def held_tensors(self):
         return super().held_tensors() + self.left.held_tensors() + self.right.held_tensors()
 
