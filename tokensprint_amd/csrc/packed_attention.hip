@@ -7,7 +7,13 @@ int launch_packed_bf16(const PackedArgs& args, bool coop, hipStream_t stream) {
 
 int ts_check_attention_args(const AttentionArgs& a, const char* who);
 
-// `coop`: a workgroup per item and share of its keys, else a wavefront per item.
+// Workgroups of the kernel that shares keys out which the card holds at a time.
+extern "C" int ts_packed_resident(int hd, int type) {
+  const int nb = pack_slices(hd);
+  return compute_units() * (type == TS_BF16 && nb <= 4 ? 2 : 1);
+}
+
+// `coop`: all items' keys shared out over `workgroups` workgroups, else a wavefront per item.
 extern "C" int ts_packed_attention(const PackedArgs* p, int type, int coop, hipStream_t stream) {
   const PackedArgs& args = *p;
   const AttentionArgs& a = args.base;
@@ -22,10 +28,8 @@ extern "C" int ts_packed_attention(const PackedArgs* p, int type, int coop, hipS
     TS_FAIL("packed_attention: without a tile list there is one token per entry");
   if ((int64_t)args.num_tiles * a.nkv * args.head_blocks > 1 << 30) TS_FAIL("packed_attention: too many tiles");
   if (coop) {
-    if (args.num_splits < 1 || args.num_splits > 65535) TS_FAIL("packed_attention: num_splits=%d", args.num_splits);
-    if (args.span < 128 || args.span % 128) TS_FAIL("packed_attention: shares of %d keys", args.span);
-    if (args.num_splits > 1 && (!args.partial_o || !args.partial_ml || !args.arrivals))
-      TS_FAIL("packed_attention: shares need partial buffers and arrival counts");
+    if (args.workgroups < 1 || !args.partial_o || !args.partial_ml || !args.arrivals)
+      TS_FAIL("packed_attention: %d workgroups need partial buffers and arrival counts", args.workgroups);
   }
   if (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages | (uintptr_t)args.partial_ml) & 15)
     TS_FAIL("packed_attention: tensors must be 16-byte aligned");

@@ -4,15 +4,18 @@
 // As over a wider cache (attention_core.h) a wavefront owns 16 query rows and takes 32 keys at a time,
 //     S^T = K Q^T,    O^T = V^T P^T         (v_mfma_f32_16x16x32_bf16),
 // a lane's scores being in place its part of the second product's operand.  Here the operands of K and V are
-// codes, turned into the bfloat16 numbers 16 + c, which are exact, and steps stand outside the products:
+// codes, turned into the numbers 16 + c, which are exact, and steps stand outside the products:
 //     q . k  =  sum over groups of  step (q . (16 + c) - (16 + zero) sum(q))
 //     o      =  sum over keys of    (p step) (16 + c) - (p step) (16 + zero)
 // Sums of q over a group are float32 numbers of a query row, that is of a lane, and start the group's product as
-// -(16 + zero) sum(q); p step is rounded to bfloat16 once and meets codes and -(16 + zero) (a product with the same number in
-// every row) alike, so what its rounding costs is in proportion to the value.  PARTS = 3 (float32 activations): q and
-// p step in three bfloat16 parts, which hold all their bits.
-// A wavefront dequantises nothing: seven instructions make a word of eight codes operands, a score costs a
-// multiplication a group and so does a weight.
+// -(16 + zero) sum(q); p step is rounded to float16 once and meets codes and -(16 + zero) (a product with the same numbers in
+// every row) alike, so what its rounding costs is in proportion to the value.
+// A wavefront dequantises nothing: seven instructions make a word of eight codes operands, a score costs two
+// multiplications a group and a weight one.
+//
+// PARTS = 3 (float32 activations): q and p step in three bfloat16 parts, which hold all their bits, against the whole numbers
+// c - zero, so that nothing cancels but what does in exact arithmetic either (with 16 + c the sums of values are of up
+// to 31 steps where the result is of a tenth of one, and 2.7e-6 off where float32 sums are 3.5e-7).
 #pragma once
 #include "attention_core.h"
 #include "packed_kv.h"
@@ -22,33 +25,59 @@ typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 struct PackedArgs {
   AttentionArgs base;        // k_pages, v_pages: blocks
   const int* tiles;          // [num_tiles, 3]: batch entry, first flat token, tokens in tile; or null: tile = entry = token
-  float* partial_o;          // [items, num_splits, 16, 32 NB]   (num_splits > 1)
-  float* partial_ml;         // [items, num_splits, 16, 2]
-  unsigned* arrivals;        // [items] zeros: the last workgroup of an item merges its splits and leaves a zero
+  float* partial_o;          // [workgroups, 2, 16, 32 NB]
+  float* partial_ml;         // [workgroups, 2, 16, 2]
+  unsigned* arrivals;        // [items] zeros: the last workgroup of an item merges its parts and leaves a zero
   int num_tiles;
   int rows_per_token;        // query heads of a tile per token: min(group, 16)
   int head_blocks;           // ceil(group / 16)
-  int num_splits;            // shares of an item's keys, of `span` keys each
-  int span;                  // a multiple of 128
+  int workgroups;            // that share all items' keys out
 };
 
 template <int NB>
 struct PackedBlock {
   static constexpr int G = pack_groups(NB * 32);
   unsigned k[2][NB], v[2][NB];
-  u32x4 ks[2][G], vs[2][G];        // steps and biases of tokens 4 g + i
+  unsigned ks[2], vs[2];           // word r % (4 G) of the steps and biases of tokens 4 g + i
+  unsigned short kz[2][G];         // PARTS = 3: the bias of token r
+  int page[2];                     // below 0: no keys there (the context ends, or a window has let go)
 };
 
-// Eight codes as the bfloat16 numbers 16 + c: codes 0 and 4, 1 and 5, 2 and 6, 3 and 7.
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
+// Eight codes as the numbers 16 + c: codes 0 and 4, 1 and 5, 2 and 6, 3 and 7 of a word of keys (bfloat16) or of
+// values (float16).
+template <bool VALUES>
 __device__ __forceinline__ void packed_codes(unsigned word, unsigned (&out)[4]) {
   // (one of the two constants in a vector register, one in a scalar: `and` and `or` are one instruction then)
-  unsigned bits = 0x00780078u, lead = 0x41804180u;
+  unsigned bits = VALUES ? 0x03c003c0u : 0x00780078u, lead = VALUES ? 0x4c004c00u : 0x41804180u;
   asm("" : "+v"(bits));
   asm("" : "+s"(lead));
   out[0] = (word & bits) | lead;
   out[1] = (word >> 4 & bits) | lead;
-  out[2] = (word >> 8 & bits) | lead;
+  out[2] = ((VALUES ? __builtin_amdgcn_alignbit(word, word, 8) : word >> 8) & bits) | lead;
   out[3] = (__builtin_amdgcn_alignbit(word, word, 12) & bits) | lead;
+}
+// Two float16 numbers as bfloat16 (whole numbers below 32: exact).
+__device__ __forceinline__ unsigned as_bf16(f16x2 x) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  return __builtin_bit_cast(unsigned, bf16x2{(bf16_t)(float)x[0], (bf16_t)(float)x[1]});
+}
+// The whole numbers code - zero of a word of keys, in bfloat16, with the bias of their token.
+__device__ __forceinline__ void whole_keys(unsigned word, _Float16 bias, unsigned (&out)[4]) {
+  unsigned c[4];
+  packed_codes<true>(__builtin_amdgcn_alignbit(word, word, 32 - (kPackTurnV - kPackTurnK)), c);
+  const f16x2 b = {bias, bias};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = as_bf16(__builtin_bit_cast(f16x2, c[i]) + b);
+}
+// The same of a word of values, with the biases of tokens 0 and 1, 2 and 3.
+__device__ __forceinline__ void whole_values(unsigned word, f16x2 b01, f16x2 b23, unsigned (&out)[4]) {
+  unsigned c[4];
+  packed_codes<true>(word, c);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = as_bf16(__builtin_bit_cast(f16x2, c[i]) + (i % 2 ? b23 : b01));
 }
 
 __device__ __forceinline__ bf16x8 as_bf16x8(unsigned a, unsigned b, unsigned c, unsigned d) {
@@ -59,10 +88,14 @@ __device__ __forceinline__ bf16x8 as_bf16x8(unsigned a, unsigned b, unsigned c, 
 // Number j of eight float16 in four words, and its product with a float32 in one instruction (of
 // the form that adds a float32: a multiplication alone would convert first).
 __device__ __forceinline__ _Float16 half_of(const u32x4& words, int j) {
-  typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
   return __builtin_bit_cast(f16x8, words)[j];
 }
 __device__ __forceinline__ float half_times(_Float16 h, float x) { return __builtin_fmaf((float)h, x, 0.f); }
+
+__device__ __forceinline__ f16x8 as_f16x8(unsigned a, unsigned b, unsigned c, unsigned d) {
+  const u32x4 v = {a, b, c, d};
+  return __builtin_bit_cast(f16x8, v);
+}
 
 template <int N>
 __device__ __forceinline__ void load_words(unsigned (&w)[N], const unsigned char* p) {
@@ -72,34 +105,52 @@ __device__ __forceinline__ void load_words(unsigned (&w)[N], const unsigned char
 
 // The 32 keys at walk coordinate `v`; calls come in steps of `stride` keys (the cursor holds this
 // call's pages and then fetches those of v + stride).
-template <int NB>
+template <int NB, int PARTS>
 __device__ __forceinline__ void load_packed(PackedBlock<NB>& b, const AttentionArgs& a, PageCursor& cur, int kvh, int v,
                                             int stride, int lane) {
   constexpr int G = PackedBlock<NB>::G, BYTES = pack_block_bytes(NB * 32), CODES = pack_codes_bytes(NB * 32);
   const int r = lane % 16, g = lane / 16, kb = cur.walk.real(v), P = a.page_size;
   const int page[2] = {cur.next0, cur.next1};
+  // offsets of 32 bits beside scalar addresses (made known here: hoisted out of the walk they would be widened, and
+  // every load would add 64 bits for itself)
+  unsigned at_code = (unsigned)(lane * (NB * 4)), at_s = (unsigned)(CODES + g * G * 16 + r % (4 * G) * 4);
+  unsigned at_z = (unsigned)(CODES + r / 4 * G * 16 + 8 + r % 4 * 2);
+  asm volatile("" : "+v"(at_code), "+v"(at_s), "+v"(at_z));
 #pragma unroll
   for (int blk = 0; blk < 2; ++blk) {
     const int64_t at = (((int64_t)max(page[blk], 0) * a.nkv + kvh) * P + ((kb + blk * 16) & (P - 1))) / 16 * BYTES;
     const unsigned char* kp = (const unsigned char*)a.k_pages + at;
     const unsigned char* vp = (const unsigned char*)a.v_pages + at;
-    load_words<NB>(b.k[blk], kp + (r * 4 + g) * (NB * 4));
-    load_words<NB>(b.v[blk], vp + lane * (NB * 4));
+    b.ks[blk] = *(const unsigned*)(kp + at_s);
+    load_words<NB>(b.k[blk], kp + at_code);
+    b.vs[blk] = *(const unsigned*)(vp + at_s);
+    load_words<NB>(b.v[blk], vp + at_code);
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      b.ks[blk][i] = *(const u32x4*)(kp + CODES + (g * G + i) * 16);
-      b.vs[blk][i] = *(const u32x4*)(vp + CODES + (g * G + i) * 16);
-    }
+    for (int i = 0; i < G; ++i)
+      if constexpr (PARTS > 1) b.kz[blk][i] = *(const unsigned short*)(kp + at_z + i * 16);
   }
-  if (page[0] < 0 || page[1] < 0) {      // where the context ends or a window has let go: steps of zero
-    const u32x4 zero = {0, 0, 0, 0};
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-      for (int i = 0; i < G; ++i)
-        if (page[blk] < 0) b.ks[blk][i] = b.vs[blk][i] = zero;
-  }
+  // (no load under a condition, which would put waits for those under way behind it: of a page that is not there, the
+  // first page's, and the mask takes its keys out)
+  b.page[0] = page[0], b.page[1] = page[1];
   cur.start(v + stride);
+}
+
+// A group's steps and biases, out of the sixteen lanes that hold a quarter's: one instruction a word.  (Loaded by every
+// lane for itself they were eight loads of 16 bytes a lane for 32 keys, and what a compute unit takes of loads, a kilobyte in
+// 7 ns, was two thirds of a walk.)
+template <int I>
+__device__ __forceinline__ u32x4 packed_scale(unsigned word) {
+  return u32x4{(unsigned)__builtin_amdgcn_update_dpp(0, (int)word, 0x150 + 4 * I, 0xf, 0xf, false),
+               (unsigned)__builtin_amdgcn_update_dpp(0, (int)word, 0x151 + 4 * I, 0xf, 0xf, false),
+               (unsigned)__builtin_amdgcn_update_dpp(0, (int)word, 0x152 + 4 * I, 0xf, 0xf, false),
+               (unsigned)__builtin_amdgcn_update_dpp(0, (int)word, 0x153 + 4 * I, 0xf, 0xf, false)};
+}
+template <int G>
+__device__ __forceinline__ u32x4 packed_scale_of(unsigned word, int i) {      // i: known when unrolled
+  if (G == 1 || i == 0) return packed_scale<0>(word);
+  if (i == 1) return packed_scale<1>(word);
+  if (i == 2) return packed_scale<2>(word);
+  return packed_scale<3>(word);
 }
 
 template <int NB, int PARTS>
@@ -169,20 +220,24 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, PARTS>& t, const Pa
   for (int blk = 0; blk < 2; ++blk) {
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      f32x4 acc;
+      const u32x4 scale = packed_scale_of<PackedBlock<NB>::G>(b.ks[blk], i);
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (PARTS == 1) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = half_times(half_of(b.ks[blk][i], 4 + j), t.qsum[i]);
+        for (int j = 0; j < 4; ++j) acc[j] = half_times(half_of(scale, 4 + j), t.qsum[i]);
+      }
 #pragma unroll
       for (int s = 2 * i; s < 2 * i + 2 && s < NB; ++s) {
         unsigned c[4];
-        packed_codes(b.k[blk][s], c);
+        if constexpr (PARTS == 1) packed_codes<false>(b.k[blk][s], c);
+        else whole_keys(b.k[blk][s], __builtin_bit_cast(_Float16, b.kz[blk][i]), c);
         const bf16x8 k = as_bf16x8(c[0], c[1], c[2], c[3]);
 #pragma unroll
         for (int p = PARTS - 1; p >= 0; --p) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, t.q[p][s], acc, 0, 0, 0);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        st[blk][j] = fmaf((float)half_of(b.ks[blk][i], j), acc[j], i == 0 ? 0.f : st[blk][j]);
+        st[blk][j] = fmaf((float)half_of(scale, j), acc[j], i == 0 ? 0.f : st[blk][j]);
     }
   }
   if constexpr (EXTRA) {
@@ -192,14 +247,14 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, PARTS>& t, const Pa
       for (int j = 0; j < 4; ++j) st[blk][j] = extra_score_log2(*x, st[blk][j], kb + blk * 16 + g * 4 + j);
     scale_log2 = 1.f;
   }
-  if (!interior) {
+  if (!interior || (b.page[0] | b.page[1]) < 0) {
     asm volatile("" ::: "memory");       // keeps this a branch
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = kb + blk * 16 + g * 4 + j;
-        st[blk][j] = (key <= t.pos && (key >= t.lo || key < t.keep)) ? st[blk][j] : -INFINITY;
+        st[blk][j] = (b.page[blk] >= 0 && key <= t.pos && (key >= t.lo || key < t.keep)) ? st[blk][j] : -INFINITY;
       }
   }
   const float mx = max2(max2(max2(max2(st[0][0], st[0][1]), st[0][2]), max2(max2(st[0][3], st[1][0]), st[1][1])),
@@ -220,31 +275,47 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, PARTS>& t, const Pa
     for (int db = 0; db < 2 * NB; ++db)
 #pragma unroll
       for (int j = 0; j < 4; ++j) t.o[db][j] *= corr;
+    if constexpr (PARTS == 1) {
 #pragma unroll
-    for (int i = 0; i < NG; ++i)
+      for (int i = 0; i < NG; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) t.oz[i][j] *= corr;
+        for (int j = 0; j < 4; ++j) t.oz[i][j] *= corr;
+    }
   }
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
-    float w[8];
+    const u32x4 s0 = packed_scale_of<PackedBlock<NB>::G>(b.vs[0], i), s1 = packed_scale_of<PackedBlock<NB>::G>(b.vs[1], i);
+    if constexpr (PARTS == 1) {
+      // (a multiplication and its rounding to float16 are one instruction)
+      f16x8 w;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = half_times(half_of(b.vs[j / 4][i], j % 4), p[j]);
-    bf16x8 part[PARTS];
-    split_parts<PARTS, float>(part, w);
-    const bf16x8 bias = as_bf16x8(b.vs[0][i][2], b.vs[0][i][3], b.vs[1][i][2], b.vs[1][i][3]);
+      for (int j = 0; j < 8; ++j) w[j] = (_Float16)half_times(half_of(j < 4 ? s0 : s1, j % 4), p[j]);
+      t.oz[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(s0[2], s0[3], s1[2], s1[3]), w, t.oz[i], 0, 0, 0);
 #pragma unroll
-    for (int q = 0; q < PARTS; ++q) t.oz[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias, part[q], t.oz[i], 0, 0, 0);
+      for (int s = 2 * i; s < 2 * i + 2 && s < NB; ++s) {
+        unsigned c[4], d[4];
+        packed_codes<true>(b.v[0][s], c);
+        packed_codes<true>(b.v[1][s], d);
+        t.o[2 * s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(c[0], c[1], d[0], d[1]), w, t.o[2 * s], 0, 0, 0);
+        t.o[2 * s + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(c[2], c[3], d[2], d[3]), w, t.o[2 * s + 1], 0, 0, 0);
+      }
+    } else {
+      float w[8];
 #pragma unroll
-    for (int s = 2 * i; s < 2 * i + 2 && s < NB; ++s) {
-      unsigned c[4], d[4];
-      packed_codes(b.v[0][s], c);
-      packed_codes(b.v[1][s], d);
-      const bf16x8 even = as_bf16x8(c[0], c[1], d[0], d[1]), odd = as_bf16x8(c[2], c[3], d[2], d[3]);
+      for (int j = 0; j < 8; ++j) w[j] = half_times(half_of(j < 4 ? s0 : s1, j % 4), p[j]);
+      bf16x8 part[PARTS];
+      split_parts<PARTS, float>(part, w);
 #pragma unroll
-      for (int q = 0; q < PARTS; ++q) {
-        t.o[2 * s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, part[q], t.o[2 * s], 0, 0, 0);
-        t.o[2 * s + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, part[q], t.o[2 * s + 1], 0, 0, 0);
+      for (int s = 2 * i; s < 2 * i + 2 && s < NB; ++s) {
+        unsigned c[4], d[4];
+        whole_values(b.v[0][s], f16x2{half_of(s0, 4), half_of(s0, 5)}, f16x2{half_of(s0, 6), half_of(s0, 7)}, c);
+        whole_values(b.v[1][s], f16x2{half_of(s1, 4), half_of(s1, 5)}, f16x2{half_of(s1, 6), half_of(s1, 7)}, d);
+        const bf16x8 even = as_bf16x8(c[0], c[1], d[0], d[1]), odd = as_bf16x8(c[2], c[3], d[2], d[3]);
+#pragma unroll
+        for (int q = PARTS - 1; q >= 0; --q) {
+          t.o[2 * s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, part[q], t.o[2 * s], 0, 0, 0);
+          t.o[2 * s + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, part[q], t.o[2 * s + 1], 0, 0, 0);
+        }
       }
     }
   }
@@ -253,97 +324,135 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, PARTS>& t, const Pa
 // The rows' sums with what the zeros take off.
 template <int NB, int PARTS>
 __device__ __forceinline__ void packed_finish(PackedTile<NB, PARTS>& t) {
+  if constexpr (PARTS == 1) {
 #pragma unroll
-  for (int db = 0; db < 2 * NB; ++db)
+    for (int db = 0; db < 2 * NB; ++db)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) t.o[db][j] += t.oz[db / 4][j];
+      for (int j = 0; j < 4; ++j) t.o[db][j] += t.oz[db / 4][j];
+  }
   t.l = col4_sum(t.l);
 }
 
-// COOP: a workgroup of four wavefronts per item and share of its keys, each every fourth block of 32 keys, merged in
-// LDS; else a wavefront per item, which walks its keys alone (prompts: tiles enough to fill the chip).
-// Shares are of `span` keys at fixed places from the item's first key on, so that requests of unlike lengths
-// give workgroups of like lengths; the last of an item's workgroups to finish merges its shares.
-template <int NB, int PARTS, bool COOP, bool EXTRA, typename T>
+constexpr int kPackedChunk = 128;      // keys: a block for each of a workgroup's wavefronts
+
+// One tile's query rows and how far they see.
+struct PackedItem {
+  int entry, tok0, ntok, pos_first, pos_last;
+  KeyWalk walk;
+  __device__ __forceinline__ int chunks() const { return (pos_last - walk.origin) / kPackedChunk + 1; }
+};
+__device__ __forceinline__ PackedItem packed_item(const PackedArgs& args, int tile) {
+  PackedItem it;
+  it.entry = args.tiles ? args.tiles[tile * 3] : tile;
+  it.tok0 = args.tiles ? args.tiles[tile * 3 + 1] : tile;
+  it.ntok = args.tiles ? args.tiles[tile * 3 + 2] : 1;
+  it.pos_first = args.base.positions[it.tok0];                // positions are consecutive
+  it.pos_last = it.pos_first + it.ntok - 1;
+  it.walk = key_walk<32>(args.base, first_visible(args.base, it.pos_first));
+  return it;
+}
+
+// The sum over the lanes up to this one.
+__device__ __forceinline__ int lanes_before(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int other = __shfl_up(v, o, kWave);
+    if (lane >= o) v += other;
+  }
+  return v;
+}
+
+// An item is a tile and a key/value head (and a block of 16 of its query heads); the chunks of 128 keys of
+// all items, one behind the other, are shared out evenly: every workgroup walks as many, whatever the lengths of the
+// requests, of one item or of several.  The lengths are on the device only (a captured step's), so every wavefront adds
+// them up for itself.  (A workgroup per item and share of at most 2,048 keys: 64 requests of 128 to 4,096 tokens 50 us, the chip
+// half empty behind the longest.)
+// A workgroup's four wavefronts take every fourth block of 32 keys and merge in LDS.  An item that ends in another
+// workgroup than it began in leaves its parts in memory, two places a workgroup (the part that an earlier one began, the
+// part that a later one goes on with), and whoever comes last merges them in their order.
+template <int NB, int PARTS, bool EXTRA, typename T>
 __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_attention_kernel(PackedArgs args) {
   constexpr int HD = 32 * NB, DB = 2 * NB;
+  constexpr int kRow = HD + 4;                                // neighbouring rows start four banks apart
+  __shared__ float s_ml[4][16][2];
+  __shared__ __attribute__((aligned(16))) float s_o[4][16][kRow];
+  __shared__ unsigned s_before;
   const AttentionArgs& a = args.base;
   const int wave = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int r = lane % 16, g = lane / 16;
-  const int group = a.nq / a.nkv;
-  const int items = args.num_tiles * a.nkv * args.head_blocks;
-  const int item = COOP ? blockIdx.x : blockIdx.x * 4 + wave;
-  if (item >= items) return;
-  const int hb = item % args.head_blocks, kvh = item / args.head_blocks % a.nkv;
-  const int tile = item / args.head_blocks / a.nkv;
-  const int entry = args.tiles ? uniform(args.tiles[tile * 3]) : tile,
-            tok0 = args.tiles ? uniform(args.tiles[tile * 3 + 1]) : tile,
-            ntok = args.tiles ? uniform(args.tiles[tile * 3 + 2]) : 1;
-  const int* table = a.table + (int64_t)entry * a.table_width;
-  const int ti = r / args.rows_per_token;
-  const int hh = hb * 16 + r % args.rows_per_token;          // head inside the group
-  const bool row_ok = ti < ntok && hh < group;
-  const int token = tok0 + min(ti, ntok - 1);
-  const int head = kvh * group + min(hh, group - 1);
-
-  const int pos_first = uniform(a.positions[tok0]);           // positions are consecutive
-  const int pos_last = pos_first + ntok - 1;
-  const KeyWalk walk = key_walk<32>(a, first_visible(a, pos_first));
-  const int share = COOP ? blockIdx.y : 0;
-  const int first = COOP ? walk.origin + share * args.span : walk.origin;
-  const int used = COOP ? min(args.num_splits, (pos_last - walk.origin) / args.span + 1) : 1;
-  if (share >= used) return;                                  // an item with fewer shares than others
-  // (the last share takes what more there is: positions beyond what the host planned for)
-  const int key_end = share == used - 1 ? pos_last + 1 : first + args.span;
-  constexpr int kStride = COOP ? 128 : 32;
-  const int key_begin = first + (COOP ? wave * 32 : 0);
-
-  PageCursor cur{(ConstTable)table, a.page_size, pos_last, walk, -1, -1};
-  cur.start(key_begin);
-  PackedBlock<NB> A, B;
-  if (key_begin < key_end) load_packed<NB>(A, a, cur, kvh, key_begin, kStride, lane);
-  PackedTile<NB, PARTS> t;
-  t.pos = row_ok ? pos_first + ti : -1;
-  t.lo = first_visible(a, t.pos);
-  t.keep = a.keep;
-  load_packed_query<NB, PARTS, T>(t, (const T*)a.q + ((int64_t)token * a.nq + head) * a.hd, row_ok, a.hd, g);
+  const int group = a.nq / a.nkv, heads = a.nkv * args.head_blocks;
   const float scale_log2 = a.scale * 1.44269504088896341f;
-  ScoreExtraLog2 x;
-  if (EXTRA) x = in_log2(score_extra(a, head, t.pos));
-  const int lo_last = first_visible(a, pos_last);
-  auto update = [&](const PackedBlock<NB>& b, int v) {
-    const int kb = walk.real(v);
-    packed_update<NB, PARTS, EXTRA>(t, b, kb, scale_log2, kb + 31 <= pos_first && kb >= lo_last, g, &x);
-  };
-  for (int v = key_begin; v < key_end; v += 2 * kStride) {
-    if (v + kStride < key_end) load_packed<NB>(B, a, cur, kvh, v + kStride, kStride, lane);
-    update(A, v);
-    if (v + kStride >= key_end) break;
-    if (v + 2 * kStride < key_end) load_packed<NB>(A, a, cur, kvh, v + 2 * kStride, kStride, lane);
-    update(B, v + kStride);
-  }
-  packed_finish<NB, PARTS>(t);
   T* out = (T*)a.out;
 
-  if constexpr (!COOP) {
-    if (!row_ok) return;
-    const float sum = sum_with_sink(t.l, t.m, a.sink, head), inv = sum > 0.f ? 1.f / sum : 0.f;
-    typedef T four __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      if (db * 16 >= a.hd) break;
-      four v;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = from_f32<T>(t.o[db][j] * inv);
-      *(four*)(out + ((int64_t)token * a.nq + head) * a.hd + db * 16 + g * 4) = v;
+  // this workgroup's chunks [at, end) of all, and the tile in which they begin
+  int total = 0;
+  for (int t0 = 0; t0 < args.num_tiles; t0 += kWave) {
+    const int n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).chunks() * heads : 0;
+    total += uniform(__shfl(lanes_before(n, lane), kWave - 1, kWave));
+  }
+  const int len = (total + args.workgroups - 1) / args.workgroups;
+  int at = blockIdx.x * len;
+  const int end = min(at + len, total);
+  if (at >= end) return;
+  int tile = 0, tile_at = 0;                                  // the tile, and its first chunk among all
+  for (int t0 = 0, sum = 0; t0 < args.num_tiles; t0 += kWave) {
+    const int n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).chunks() * heads : 0;
+    const int upto = sum + lanes_before(n, lane);
+    const unsigned long long here = __builtin_amdgcn_ballot_w64(upto > at);
+    if (here != 0) {
+      const int l = __builtin_ctzll(here);
+      tile = t0 + l;
+      tile_at = uniform(__shfl(upto - n, l, kWave));
+      break;
     }
-    return;
-  } else {
+    sum = uniform(__shfl(upto, kWave - 1, kWave));
+  }
+
+  while (at < end) {
+    PackedItem it = packed_item(args, uniform(tile));
+    it.entry = uniform(it.entry), it.tok0 = uniform(it.tok0), it.ntok = uniform(it.ntok);
+    it.pos_first = uniform(it.pos_first), it.pos_last = uniform(it.pos_last);
+    it.walk.begin = uniform(it.walk.begin), it.walk.origin = uniform(it.walk.origin);
+    const int chunks = it.chunks(), head_of = (at - tile_at) / chunks, first_chunk = at - tile_at - head_of * chunks;
+    const int count = min(chunks - first_chunk, end - at);
+    const int item_at = at - first_chunk, item = tile * heads + head_of;
+    const int hb = head_of % args.head_blocks, kvh = head_of / args.head_blocks;
+    at += count;
+    if (at == tile_at + chunks * heads) { tile_at = at; ++tile; }
+
+    const int* table = a.table + (int64_t)it.entry * a.table_width;
+    const int ti = r / args.rows_per_token;
+    const int hh = hb * 16 + r % args.rows_per_token;        // head inside the group
+    const bool row_ok = ti < it.ntok && hh < group;
+    const int token = it.tok0 + min(ti, it.ntok - 1), head = kvh * group + min(hh, group - 1);
+    const int key_begin = it.walk.origin + first_chunk * kPackedChunk + wave * 32;
+    const int key_end = min(it.walk.origin + (first_chunk + count) * kPackedChunk, it.pos_last + 1);
+    PageCursor cur{(ConstTable)table, a.page_size, it.pos_last, it.walk, -1, -1};
+    cur.start(key_begin);
+    PackedBlock<NB> A, B;
+    load_packed<NB, PARTS>(A, a, cur, kvh, key_begin, kPackedChunk, lane);
+    PackedTile<NB, PARTS> t;
+    t.pos = row_ok ? it.pos_first + ti : -1;
+    t.lo = first_visible(a, t.pos);
+    t.keep = a.keep;
+    load_packed_query<NB, PARTS, T>(t, (const T*)a.q + ((int64_t)token * a.nq + head) * a.hd, row_ok, a.hd, g);
+    ScoreExtraLog2 x;
+    if (EXTRA) x = in_log2(score_extra(a, head, t.pos));
+    const int lo_last = first_visible(a, it.pos_last);
+    auto update = [&](const PackedBlock<NB>& b, int v) {
+      const int kb = it.walk.real(v);
+      packed_update<NB, PARTS, EXTRA>(t, b, kb, scale_log2, kb + 31 <= it.pos_first && kb >= lo_last, g, &x);
+    };
+    for (int v = key_begin; v < key_end; v += 2 * kPackedChunk) {
+      load_packed<NB, PARTS>(B, a, cur, kvh, v + kPackedChunk, kPackedChunk, lane);
+      update(A, v);
+      if (v + kPackedChunk >= key_end) break;
+      load_packed<NB, PARTS>(A, a, cur, kvh, v + 2 * kPackedChunk, kPackedChunk, lane);
+      update(B, v + kPackedChunk);
+    }
+    packed_finish<NB, PARTS>(t);
+
     // the wavefronts' results through LDS, an element at a time to a thread (rows that exist only)
-    constexpr int kRow = HD + 4;                              // neighbouring rows start four banks apart
-    __shared__ float s_ml[4][16][2];
-    __shared__ __attribute__((aligned(16))) float s_o[4][16][kRow];
-    __shared__ unsigned s_before;
     if (g == 0) {
       s_ml[wave][r][0] = t.m;
       s_ml[wave][r][1] = t.l;
@@ -351,17 +460,18 @@ __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_att
 #pragma unroll
     for (int db = 0; db < DB; ++db) *(f32x4*)&s_o[wave][r][db * 16 + g * 4] = t.o[db];
     __syncthreads();
-    const int rows = ntok * args.rows_per_token;              // the last row of a tile of several tokens; heads past
-    const int64_t slot0 = ((int64_t)item * args.num_splits + share) * 16;      // the group's are not stored
-    const bool alone = used == 1;
-    auto place = [&](int row) -> int64_t {                    // of a row's result, or -1
+    const int rows = it.ntok * args.rows_per_token;
+    const bool whole = count == chunks;
+    const int64_t slot0 = ((int64_t)blockIdx.x * 2 + (first_chunk == 0 ? 1 : 0)) * 16;
+    auto place = [&](int row) -> int64_t {                    // of a row's result, or -1: no such head
       const int rt = row / args.rows_per_token, rh = hb * 16 + row % args.rows_per_token;
-      return rh < group ? ((int64_t)(tok0 + rt) * a.nq + kvh * group + rh) * a.hd : -1;
+      return rh < group ? ((int64_t)(it.tok0 + rt) * a.nq + kvh * group + rh) * a.hd : -1;
     };
+    auto sink_of = [&](int row) { return kvh * group + hb * 16 + row % args.rows_per_token; };
     for (int e = threadIdx.x; e < rows * HD; e += 256) {
       const int row = e / HD, d = e % HD;
-      const int64_t at = place(row);
-      if (at < 0 || d >= a.hd) continue;
+      const int64_t to = place(row);
+      if (to < 0 || d >= a.hd) continue;
       float M = s_ml[0][row][0];
 #pragma unroll
       for (int w = 1; w < 4; ++w) M = fmaxf(M, s_ml[w][row][0]);
@@ -373,9 +483,9 @@ __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_att
         sum = fmaf(s_ml[w][row][1], ww, sum);
         acc = fmaf(s_o[w][row][d], ww, acc);
       }
-      if (alone) {
-        sum = sum_with_sink(sum, M, a.sink, kvh * group + hb * 16 + row % args.rows_per_token);
-        out[at + d] = from_f32<T>(acc * (sum > 0.f ? 1.f / sum : 0.f));
+      if (whole) {
+        sum = sum_with_sink(sum, M, a.sink, sink_of(row));
+        out[to + d] = from_f32<T>(acc * (sum > 0.f ? 1.f / sum : 0.f));
       } else {
         __hip_atomic_store(args.partial_o + (slot0 + row) * HD + d, acc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (d == 0)
@@ -384,50 +494,112 @@ __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_att
                              __HIP_MEMORY_SCOPE_AGENT);
       }
     }
-    if (alone) return;
-    // The shares' results pass the caches that another XCD does not share; each wave waits until its own have
-    // been taken, the workgroup counts itself in, and the one that finds all others there merges.
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (threadIdx.x == 0)
-      s_before = __hip_atomic_fetch_add(args.arrivals + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if ((int)s_before + 1 != used) return;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-    if (threadIdx.x == 0) __hip_atomic_store(args.arrivals + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int e = threadIdx.x; e < rows * HD; e += 256) {
-      const int row = e / HD, d = e % HD;
-      const int64_t at = place(row);
-      if (at < 0 || d >= a.hd) continue;
-      float M = -INFINITY, sum = 0.f, acc = 0.f;
-      for (int s0 = 0; s0 < used; s0 += 4) {                  // four at a time: everything asked for before its use
-        float ms[4], ls[4], part[4];
+    if (!whole) {
+      // The parts' results pass the caches that another XCD does not share; each wave waits until its own have
+      // been taken, the workgroup counts itself in, and the one that finds all others there merges.
+      const int first_wg = item_at / len, parts = (item_at + chunks - 1) / len - first_wg + 1;
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      if (threadIdx.x == 0)
+        s_before = __hip_atomic_fetch_add(args.arrivals + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if ((int)s_before + 1 == parts) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+        if (threadIdx.x == 0) __hip_atomic_store(args.arrivals + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int e = threadIdx.x; e < rows * HD; e += 256) {
+          const int row = e / HD, d = e % HD;
+          const int64_t to = place(row);
+          if (to < 0 || d >= a.hd) continue;
+          float M = -INFINITY, sum = 0.f, acc = 0.f;
+          for (int s0 = 0; s0 < parts; s0 += 4) {             // four at a time: everything asked for before its use
+            float ms[4], ls[4], part[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t slot = ((int64_t)item * args.num_splits + min(s0 + j, used - 1)) * 16 + row;
-          const uint64_t ml = __hip_atomic_load((const uint64_t*)args.partial_ml + slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          ms[j] = s0 + j < used ? __uint_as_float((unsigned)ml) : -INFINITY;
-          ls[j] = __uint_as_float((unsigned)(ml >> 32));
-          part[j] = __hip_atomic_load(args.partial_o + slot * HD + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int j = 0; j < 4; ++j) {
+              const int p = min(s0 + j, parts - 1);
+              const int64_t slot = ((int64_t)(first_wg + p) * 2 + (p == 0 ? 1 : 0)) * 16 + row;
+              const uint64_t ml = __hip_atomic_load((const uint64_t*)args.partial_ml + slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+              ms[j] = s0 + j < parts ? __uint_as_float((unsigned)ml) : -INFINITY;
+              ls[j] = __uint_as_float((unsigned)(ml >> 32));
+              part[j] = __hip_atomic_load(args.partial_o + slot * HD + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            float Mg = M;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) Mg = fmaxf(Mg, ms[j]);
+            const float Mc = Mg == -INFINITY ? 0.f : Mg, keep = __builtin_amdgcn_exp2f(M - Mc);
+            sum *= keep;
+            acc *= keep;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float w = __builtin_amdgcn_exp2f(ms[j] - Mc);
+              sum = fmaf(ls[j], w, sum);
+              acc = fmaf(part[j], w, acc);
+            }
+            M = Mg;
+          }
+          sum = sum_with_sink(sum, M, a.sink, sink_of(row));
+          out[to + d] = from_f32<T>(acc * (sum > 0.f ? 1.f / sum : 0.f));
         }
-        float Mg = M;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) Mg = fmaxf(Mg, ms[j]);
-        const float Mc = Mg == -INFINITY ? 0.f : Mg, keep = __builtin_amdgcn_exp2f(M - Mc);
-        sum *= keep;
-        acc *= keep;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float w = __builtin_amdgcn_exp2f(ms[j] - Mc);
-          sum = fmaf(ls[j], w, sum);
-          acc = fmaf(part[j], w, acc);
-        }
-        M = Mg;
       }
-      sum = sum_with_sink(sum, M, a.sink, kvh * group + hb * 16 + row % args.rows_per_token);
-      out[at + d] = from_f32<T>(acc * (sum > 0.f ? 1.f / sum : 0.f));
     }
+    if (at < end) __syncthreads();                            // everybody has read what stands in LDS
+  }
+}
+
+// A wavefront per tile and head, which walks its keys alone: tiles enough to fill the chip (prompts).
+template <int NB, int PARTS, bool EXTRA, typename T>
+__global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_walk_kernel(PackedArgs args) {
+  constexpr int DB = 2 * NB;
+  const AttentionArgs& a = args.base;
+  const int wave = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int r = lane % 16, g = lane / 16;
+  const int group = a.nq / a.nkv, heads = a.nkv * args.head_blocks;
+  const int item = blockIdx.x * 4 + wave;
+  if (item >= args.num_tiles * heads) return;
+  const int hb = item % args.head_blocks, kvh = item / args.head_blocks % a.nkv;
+  PackedItem it = packed_item(args, uniform(item / heads));
+  it.entry = uniform(it.entry), it.tok0 = uniform(it.tok0), it.ntok = uniform(it.ntok);
+  it.pos_first = uniform(it.pos_first), it.pos_last = uniform(it.pos_last);
+  it.walk.begin = uniform(it.walk.begin), it.walk.origin = uniform(it.walk.origin);
+  const int ti = r / args.rows_per_token, hh = hb * 16 + r % args.rows_per_token;
+  const bool row_ok = ti < it.ntok && hh < group;
+  const int token = it.tok0 + min(ti, it.ntok - 1), head = kvh * group + min(hh, group - 1);
+  const int key_begin = it.walk.origin, key_end = it.pos_last + 1;
+  PageCursor cur{(ConstTable)(a.table + (int64_t)it.entry * a.table_width), a.page_size, it.pos_last, it.walk, -1, -1};
+  cur.start(key_begin);
+  PackedBlock<NB> A, B;
+  load_packed<NB, PARTS>(A, a, cur, kvh, key_begin, 32, lane);
+  PackedTile<NB, PARTS> t;
+  t.pos = row_ok ? it.pos_first + ti : -1;
+  t.lo = first_visible(a, t.pos);
+  t.keep = a.keep;
+  load_packed_query<NB, PARTS, T>(t, (const T*)a.q + ((int64_t)token * a.nq + head) * a.hd, row_ok, a.hd, g);
+  ScoreExtraLog2 x;
+  if (EXTRA) x = in_log2(score_extra(a, head, t.pos));
+  const int lo_last = first_visible(a, it.pos_last);
+  auto update = [&](const PackedBlock<NB>& b, int v) {
+    const int kb = it.walk.real(v);
+    packed_update<NB, PARTS, EXTRA>(t, b, kb, a.scale * 1.44269504088896341f,
+                                    kb + 31 <= it.pos_first && kb >= lo_last, g, &x);
+  };
+  for (int v = key_begin; v < key_end; v += 64) {
+    load_packed<NB, PARTS>(B, a, cur, kvh, v + 32, 32, lane);
+    update(A, v);
+    if (v + 32 >= key_end) break;
+    load_packed<NB, PARTS>(A, a, cur, kvh, v + 64, 32, lane);
+    update(B, v + 32);
+  }
+  packed_finish<NB, PARTS>(t);
+  if (!row_ok) return;
+  const float sum = sum_with_sink(t.l, t.m, a.sink, head), inv = sum > 0.f ? 1.f / sum : 0.f;
+  typedef T four __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    if (db * 16 >= a.hd) break;
+    four v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = from_f32<T>(t.o[db][j] * inv);
+    *(four*)((T*)a.out + ((int64_t)token * a.nq + head) * a.hd + db * 16 + g * 4) = v;
   }
 }
 
@@ -435,9 +607,9 @@ template <int NB, int PARTS, bool EXTRA, typename T>
 static int launch_packed(const PackedArgs& args, bool coop, hipStream_t stream) {
   const int items = args.num_tiles * args.base.nkv * args.head_blocks;
   if (coop)
-    hipLaunchKernelGGL((packed_attention_kernel<NB, PARTS, true, EXTRA, T>), dim3(items, args.num_splits), dim3(256), 0, stream, args);
+    hipLaunchKernelGGL((packed_attention_kernel<NB, PARTS, EXTRA, T>), dim3(args.workgroups), dim3(256), 0, stream, args);
   else
-    hipLaunchKernelGGL((packed_attention_kernel<NB, PARTS, false, EXTRA, T>), dim3((items + 3) / 4), dim3(256), 0, stream, args);
+    hipLaunchKernelGGL((packed_walk_kernel<NB, PARTS, EXTRA, T>), dim3((items + 3) / 4), dim3(256), 0, stream, args);
   TS_CHECK_LAUNCH("packed_attention");
   return 0;
 }

@@ -16,17 +16,19 @@
 // A block is 16 tokens of a page and one key/value head.  Its bytes lie as the wavefront of the
 // attention kernels wants them (lane = 16 g + r): one load of 4 NB bytes a lane, NB = slices of 32 elements,
 // for all codes of the block's keys, and one for its values':
-//   keys    codes  [token r][g][NB] words: elements 32 b + 8 g + j of token r
+//   keys    codes  [g][token r][NB] words: elements 32 b + 8 g + j of token r
 //           scale  [g][G]{ step [4], bias [4] } of tokens 4 g + i (as the score product leaves the tokens): the step
-//                  and -(16 + zero), both float16
+//                  and -(16 + zero), all float16
 //   values  codes  [g][r][NB] words: elements 32 b + r and 32 b + 16 + r of tokens 4 g + i
-//           scale  the same of the values, the bias in bfloat16 (an operand of the product)
+//           scale  the same of the values
 // G: groups of a head rounded up to a power of two.  128 elements: 1,152 bytes for 16 keys, 16 values the same
 // (bfloat16: 4,096), 4.5 bits an element.
 //
 // A code c becomes the bfloat16 number 16 + c by putting its bits behind the leading bit of 16, so a word
-// gives eight operands in seven instructions: (word >> 4 i) & 0x00780078 | 0x41804180.  For that a
-// word is kept turned left by three bits.  Code p of a word (before turning: bits 4 p .. 4 p + 3) is
+// gives eight operands in seven instructions: (word >> 4 i) & 0x00780078 | 0x41804180; values the same in float16 (0x03c003c0,
+// 0x4c004c00), because a weight times a step is rounded to float16, an eighth of bfloat16's error, in the instruction that
+// multiplies (weights are at most 1 and steps float16 numbers: nothing overflows).  For that a
+// word of keys is kept turned left by three bits, one of values by six.  Code p of a word (before turning: bits 4 p .. 4 p + 3) is
 // element j = 2 p of keys for p < 4, 2 (p - 4) + 1 else; of values, token i of the first element for p = i / 2 + 4
 // (i % 2), of the second 2 further.
 #pragma once
@@ -86,5 +88,9 @@ __device__ __forceinline__ PackGroup pack_eight(float (&v)[8], unsigned (&code)[
   return p;
 }
 
-__device__ __forceinline__ unsigned pack_turned(unsigned word) { return __builtin_rotateleft32(word, 3); }
-__device__ __forceinline__ unsigned pack_unturned(unsigned word) { return __builtin_rotateright32(word, 3); }
+// How far a word of keys, and one of values, is turned.
+constexpr int kPackTurnK = 3, kPackTurnV = 6;
+template <int BY>
+__device__ __forceinline__ unsigned pack_turned(unsigned word) { return __builtin_rotateleft32(word, BY); }
+template <int BY>
+__device__ __forceinline__ unsigned pack_unturned(unsigned word) { return __builtin_rotateright32(word, BY); }

@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void pack_store_kernel(PackStoreArgs a) {
     unsigned word = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) word |= code[j] << (4 * (j / 2 + 4 * (j % 2)));
-    if (sub < NB * 4) ((unsigned*)block)[(token * 4 + sub % 4) * NB + sub / 4] = pack_turned(word);
+    if (sub < NB * 4) ((unsigned*)block)[(sub % 4 * 16 + token) * NB + sub / 4] = pack_turned<kPackTurnK>(word);
     if (sub % 8 == 0 && there) {
       _Float16* scale = (_Float16*)(block + pack_codes_bytes(hd) + (token / 4 * G + sub / 8) * 16);
       scale[token % 4] = p.step;
@@ -141,10 +141,10 @@ __global__ __launch_bounds__(256) void pack_store_kernel(PackStoreArgs a) {
     unsigned* words = (unsigned*)block + (quad * 16 + sub % 2 * 8 + second * 4) * NB + sub / 4;
     if (count < 4) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) word[e] |= pack_unturned(words[e * NB]) & ~mask;
+      for (int e = 0; e < 4; ++e) word[e] |= pack_unturned<kPackTurnV>(words[e * NB]) & ~mask;
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) words[e * NB] = pack_turned(word[e]);
+    for (int e = 0; e < 4; ++e) words[e * NB] = pack_turned<kPackTurnV>(word[e]);
   }
   if (sub % 8 == 0 && there) {
     unsigned char* scale = block + pack_codes_bytes(hd) + (quad * G + sub / 8) * 16;
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256) void pack_store_kernel(PackStoreArgs a) {
     for (int j = 0; j < 4; ++j)
       if (j < count) {
         ((_Float16*)scale)[i0 + j] = step[j];
-        ((bf16_t*)scale)[4 + i0 + j] = (bf16_t)(-16.f - zero[j]);
+        ((_Float16*)scale)[4 + i0 + j] = (_Float16)(-16.f - zero[j]);
       }
   }
 }
@@ -246,16 +246,16 @@ __global__ __launch_bounds__(256) void pack_values_kernel(const unsigned char* _
     const unsigned* words = (const unsigned*)block;
     const unsigned char* scale = block + pack_codes_bytes(hd) + (quad * G + sub / 8) * 16;
     const float step = (float)((const _Float16*)scale)[i];
-    const float zero = -16.f - (key ? (float)((const _Float16*)scale)[4 + i] : (float)((const bf16_t*)scale)[4 + i]);
+    const float zero = -16.f - (float)((const _Float16*)scale)[4 + i];
     unsigned code[8];
     if (key) {
-      const unsigned word = pack_unturned(words[(token * 4 + sub % 4) * NB + sub / 4]);
+      const unsigned word = pack_unturned<kPackTurnK>(words[(sub % 4 * 16 + token) * NB + sub / 4]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) code[j] = word >> (4 * (j / 2 + 4 * (j % 2))) & 15;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        code[e] = pack_unturned(words[(quad * 16 + sub % 2 * 8 + e) * NB + sub / 4]) >>
+        code[e] = pack_unturned<kPackTurnV>(words[(quad * 16 + sub % 2 * 8 + e) * NB + sub / 4]) >>
                   (4 * (2 * (sub / 2 % 2) + i / 2 + 4 * (i % 2))) & 15;
     }
 #pragma unroll

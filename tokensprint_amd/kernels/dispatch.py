@@ -152,10 +152,10 @@ class Dispatch:
     per_wave_workgroups: int = 4096
 
     # ---- attention over keys and values of 4 bits: up to so many tiles of 16 rows (times key/value
-    # heads) a workgroup per tile and share of its keys, above it a wavefront per tile; the
-    # workgroups that shares are made for.
+    # heads) all their keys are shared out evenly over workgroups (as many as the card holds at a
+    # time; `packed_workgroups` another number), above it a wavefront walks a tile's keys.
     packed_items: int = 2048
-    packed_workgroups: int = 1024
+    packed_workgroups: int = 0
 
     # ---- recurrences.  A step whose longest portion has more tokens than this runs in chunks of
     # 64 tokens as products of matrices, below it every entry is walked whole by one launch.

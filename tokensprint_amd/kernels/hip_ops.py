@@ -77,7 +77,7 @@ class PackedArgs(Structure):
     _fields_ = [
         ("base", AttentionArgs), ("tiles", c_void_p), ("partial_o", c_void_p),
         ("partial_ml", c_void_p), ("arrivals", c_void_p), ("num_tiles", c_int),
-        ("rows_per_token", c_int), ("head_blocks", c_int), ("num_splits", c_int), ("span", c_int),
+        ("rows_per_token", c_int), ("head_blocks", c_int), ("workgroups", c_int),
     ]
 
 
@@ -1196,18 +1196,14 @@ class HipOps:
         d = self.dispatch
         coop = items <= d.packed_items
         if coop:
-            # shares of the keys: as long as `packed_workgroups` workgroups leave them, of the
-            # longest context's
-            chunks = -(-keys // 128)
-            m.span = 128 * max(1, -(-chunks * items // d.packed_workgroups),
-                               -(-chunks // 256))
-            m.num_splits = -(-keys // m.span)
-            if m.num_splits > 1:
-                hd = -(-a.hd // 32) * 32
-                po = torch.empty(items * m.num_splits * 16 * hd, dtype=torch.float32, device=self.device)
-                pml = torch.empty(items * m.num_splits * 16 * 2, dtype=torch.float32, device=self.device)
-                m.partial_o, m.partial_ml = po.data_ptr(), pml.data_ptr()
-                m.arrivals = self._counts(items).data_ptr()
+            # a workgroup for every 128 keys that there can be, as many as the card holds at a time
+            m.workgroups = min(items * -(-keys // 128),
+                               d.packed_workgroups or self.lib.ts_packed_resident(a.hd, _TYPE_CODE[dtype]))
+            hd = -(-a.hd // 32) * 32
+            partial = torch.empty(m.workgroups * 32 * (hd + 2), dtype=torch.float32, device=self.device)
+            m.partial_o = partial.data_ptr()
+            m.partial_ml = m.partial_o + m.workgroups * 32 * hd * 4
+            m.arrivals = self._counts(items).data_ptr()
         self._call(self.lib.ts_packed_attention, byref(m), _TYPE_CODE[dtype], int(coop), self._stream())
 
     def attend(self, qkv, batch, table, cache, write_cache, *, num_heads, num_kv_heads,
