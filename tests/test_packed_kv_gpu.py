@@ -295,9 +295,9 @@ OPTIONS = {
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("spans", ["decode", "mixed"])
 @pytest.mark.parametrize("options", list(OPTIONS))
-@pytest.mark.parametrize("walk", ["shares", "one workgroup", "wavefronts"])
+@pytest.mark.parametrize("walk", ["shares", "one workgroup", "whole items", "wavefronts"])
 def test_attention_options(ops, gpu_device, dispatch, dtype, spans, options, walk):
-    dispatch(packed_items=0 if walk == "wavefronts" else 1 << 20,
+    dispatch(packed_items=0 if walk == "wavefronts" else 1 << 20, packed_whole=1 << 20 if walk == "whole items" else 0,
              packed_workgroups={"shares": 0, "one workgroup": 1}.get(walk, 7))
     kw = dict(OPTIONS[options])
     nq, nkv, hd = 6, 2, 64
@@ -314,7 +314,7 @@ def test_long_contexts_in_shares(ops, gpu_device, dispatch, dtype):
     spans = [(0, 1), (2999, 1), (1000, 1), (130, 1)]
     got = check_attention(ops, gpu_device, nq=4, nkv=2, hd=64, page=16, spans=spans, dtype=dtype)
     for workgroups in (1, 3, 24, 100, 400):
-        dispatch(packed_workgroups=workgroups)
+        dispatch(packed_workgroups=workgroups, packed_whole=0)
         again = check_attention(ops, gpu_device, nq=4, nkv=2, hd=64, page=16, spans=spans, dtype=dtype)
         twice = check_attention(ops, gpu_device, nq=4, nkv=2, hd=64, page=16, spans=spans, dtype=dtype)
         assert torch.equal(again, twice)             # the order of arrival changes nothing

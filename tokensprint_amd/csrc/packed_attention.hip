@@ -2,15 +2,14 @@
 #include "packed_attention_kernel.h"
 
 int launch_packed_bf16(const PackedArgs& args, bool coop, hipStream_t stream) {
-  TS_PACKED_CASES(1, false, bf16_t);
+  TS_PACKED_CASES(false, false, bf16_t);
 }
 
 int ts_check_attention_args(const AttentionArgs& a, const char* who);
 
 // Workgroups of the kernel that shares keys out which the card holds at a time.
 extern "C" int ts_packed_resident(int hd, int type) {
-  const int nb = pack_slices(hd);
-  return compute_units() * (type == TS_BF16 && nb <= 4 ? 2 : 1);
+  return compute_units() * packed_waves(pack_slices(hd), type == TS_F32);
 }
 
 // `coop`: all items' keys shared out over `workgroups` workgroups, else a wavefront per item.
@@ -28,7 +27,7 @@ extern "C" int ts_packed_attention(const PackedArgs* p, int type, int coop, hipS
     TS_FAIL("packed_attention: without a tile list there is one token per entry");
   if ((int64_t)args.num_tiles * a.nkv * args.head_blocks > 1 << 30) TS_FAIL("packed_attention: too many tiles");
   if (coop) {
-    if (args.workgroups < 1 || !args.partial_o || !args.partial_ml || !args.arrivals)
+    if (args.workgroups < 0 || args.workgroups > 1 << 20 || (args.workgroups && (!args.partial_o || !args.partial_ml || !args.arrivals)))
       TS_FAIL("packed_attention: %d workgroups need partial buffers and arrival counts", args.workgroups);
   }
   if (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages | (uintptr_t)args.partial_ml) & 15)

@@ -2,5 +2,5 @@
 #include "packed_attention_kernel.h"
 
 int launch_packed_bf16_scores(const PackedArgs& args, bool coop, hipStream_t stream) {
-  TS_PACKED_CASES(1, true, bf16_t);
+  TS_PACKED_CASES(false, true, bf16_t);
 }

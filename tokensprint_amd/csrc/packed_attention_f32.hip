@@ -2,5 +2,5 @@
 #include "packed_attention_kernel.h"
 
 int launch_packed_f32(const PackedArgs& args, bool coop, hipStream_t stream) {
-  TS_PACKED_CASES(3, false, float);
+  TS_PACKED_CASES(true, false, float);
 }

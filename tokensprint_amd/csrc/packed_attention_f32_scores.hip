@@ -2,5 +2,5 @@
 #include "packed_attention_kernel.h"
 
 int launch_packed_f32_scores(const PackedArgs& args, bool coop, hipStream_t stream) {
-  TS_PACKED_CASES(3, true, float);
+  TS_PACKED_CASES(true, true, float);
 }

@@ -13,9 +13,12 @@
 // A wavefront dequantises nothing: seven instructions make a word of eight codes operands, a score costs two
 // multiplications a group and a weight one.
 //
-// PARTS = 3 (float32 activations): q and p step in three bfloat16 parts, which hold all their bits, against the whole numbers
-// c - zero, so that nothing cancels but what does in exact arithmetic either (with 16 + c the sums of values are of up
-// to 31 steps where the result is of a tenth of one, and 2.7e-6 off where float32 sums are 3.5e-7).
+// WIDE (float32 activations): the whole numbers c - zero instead, so that nothing cancels but what does in exact
+// arithmetic either (with 16 + c the sums of values are of up to 31 steps where the result is of a tenth of one, and were
+// 2.7e-6 off where float32 sums are 3.5e-7), against q and p step in two float16 parts of 11 bits each.  A query row is
+// scaled by a power of two first, to stand high in float16's range; the second part of p step counts 2,048 times in sums of
+// its own.  (Three bfloat16 parts hold 24 bits, but whole numbers in bfloat16 are three more instructions for two: 26 us for 24
+// requests of up to 1,024 keys of 64, most of it instructions met for the first time.)
 #pragma once
 #include "attention_core.h"
 #include "packed_kv.h"
@@ -31,7 +34,7 @@ struct PackedArgs {
   int num_tiles;
   int rows_per_token;        // query heads of a tile per token: min(group, 16)
   int head_blocks;           // ceil(group / 16)
-  int workgroups;            // that share all items' keys out
+  int workgroups;            // that share all items' keys out; 0: a workgroup per item
 };
 
 template <int NB>
@@ -39,7 +42,7 @@ struct PackedBlock {
   static constexpr int G = pack_groups(NB * 32);
   unsigned k[2][NB], v[2][NB];
   unsigned ks[2], vs[2];           // word r % (4 G) of the steps and biases of tokens 4 g + i
-  unsigned short kz[2][G];         // PARTS = 3: the bias of token r
+  unsigned kz[2][G];               // WIDE: the bias of token r (a word of its own: halves would go through LDS)
   int page[2];                     // below 0: no keys there (the context ends, or a window has let go)
 };
 
@@ -59,25 +62,22 @@ __device__ __forceinline__ void packed_codes(unsigned word, unsigned (&out)[4]) 
   out[2] = ((VALUES ? __builtin_amdgcn_alignbit(word, word, 8) : word >> 8) & bits) | lead;
   out[3] = (__builtin_amdgcn_alignbit(word, word, 12) & bits) | lead;
 }
-// Two float16 numbers as bfloat16 (whole numbers below 32: exact).
-__device__ __forceinline__ unsigned as_bf16(f16x2 x) {
-  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-  return __builtin_bit_cast(unsigned, bf16x2{(bf16_t)(float)x[0], (bf16_t)(float)x[1]});
-}
-// The whole numbers code - zero of a word of keys, in bfloat16, with the bias of their token.
-__device__ __forceinline__ void whole_keys(unsigned word, _Float16 bias, unsigned (&out)[4]) {
+// The whole numbers code - zero of a word of keys in float16, with the bias of their token.
+__device__ __forceinline__ void whole_keys(unsigned word, unsigned bias, unsigned (&out)[4]) {
   unsigned c[4];
   packed_codes<true>(__builtin_amdgcn_alignbit(word, word, 32 - (kPackTurnV - kPackTurnK)), c);
-  const f16x2 b = {bias, bias};
+  const _Float16 bias16 = __builtin_bit_cast(_Float16, (unsigned short)bias);
+  const f16x2 b = {bias16, bias16};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = as_bf16(__builtin_bit_cast(f16x2, c[i]) + b);
+  for (int i = 0; i < 4; ++i) out[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, c[i]) + b);
 }
 // The same of a word of values, with the biases of tokens 0 and 1, 2 and 3.
 __device__ __forceinline__ void whole_values(unsigned word, f16x2 b01, f16x2 b23, unsigned (&out)[4]) {
   unsigned c[4];
   packed_codes<true>(word, c);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = as_bf16(__builtin_bit_cast(f16x2, c[i]) + (i % 2 ? b23 : b01));
+  for (int i = 0; i < 4; ++i)
+    out[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, c[i]) + (i % 2 ? b23 : b01));
 }
 
 __device__ __forceinline__ bf16x8 as_bf16x8(unsigned a, unsigned b, unsigned c, unsigned d) {
@@ -105,7 +105,7 @@ __device__ __forceinline__ void load_words(unsigned (&w)[N], const unsigned char
 
 // The 32 keys at walk coordinate `v`; calls come in steps of `stride` keys (the cursor holds this
 // call's pages and then fetches those of v + stride).
-template <int NB, int PARTS>
+template <int NB, bool WIDE>
 __device__ __forceinline__ void load_packed(PackedBlock<NB>& b, const AttentionArgs& a, PageCursor& cur, int kvh, int v,
                                             int stride, int lane) {
   constexpr int G = PackedBlock<NB>::G, BYTES = pack_block_bytes(NB * 32), CODES = pack_codes_bytes(NB * 32);
@@ -127,7 +127,7 @@ __device__ __forceinline__ void load_packed(PackedBlock<NB>& b, const AttentionA
     load_words<NB>(b.v[blk], vp + at_code);
 #pragma unroll
     for (int i = 0; i < G; ++i)
-      if constexpr (PARTS > 1) b.kz[blk][i] = *(const unsigned short*)(kp + at_z + i * 16);
+      if constexpr (WIDE) b.kz[blk][i] = *(const unsigned short*)(kp + at_z + i * 16);
   }
   // (no load under a condition, which would put waits for those under way behind it: of a page that is not there, the
   // first page's, and the mask takes its keys out)
@@ -153,56 +153,72 @@ __device__ __forceinline__ u32x4 packed_scale_of(unsigned word, int i) {      //
   return packed_scale<3>(word);
 }
 
-template <int NB, int PARTS>
+template <int NB, bool WIDE>
 struct PackedTile {
   static constexpr int NG = (NB + 1) / 2;        // groups that exist
-  bf16x8 q[PARTS][NB];
-  float qsum[NG];            // the row's sum over each group
-  f32x4 o[2 * NB], oz[NG];
+  u32x4 q[WIDE ? 2 : 1][NB]; // bfloat16, or two parts in float16
+  float qsum[NG];            // the row's sum over each group; WIDE: qsum[0] is what turns a product into q . k
+  f32x4 o[2 * NB], oz[WIDE ? 2 * NB : NG];       // oz: the zeros' share; WIDE: sums of the second parts
   float m, l;
   int pos, lo, keep;
 };
 
-template <int PARTS, typename T>
-__device__ __forceinline__ void split_parts(bf16x8 (&part)[PARTS], const T (&x)[8]) {
-  float left[8];
+// The parts of eight numbers: 11 bits, and 2^up times the next 11.
+template <int UP>
+__device__ __forceinline__ void two_parts(u32x4 (&part)[2], const float (&x)[8]) {
+  f16x8 hi, lo;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) left[j] = to_f32(x[j]);
-#pragma unroll
-  for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      part[p][j] = (bf16_t)left[j];
-      left[j] -= (float)part[p][j];
-    }
+  for (int j = 0; j < 8; ++j) {
+    hi[j] = (_Float16)x[j];
+    lo[j] = (_Float16)((x[j] - (float)hi[j]) * (float)(1 << UP));
+  }
+  part[0] = __builtin_bit_cast(u32x4, hi);
+  part[1] = __builtin_bit_cast(u32x4, lo);
 }
 
-template <int NB, int PARTS, typename T>
-__device__ __forceinline__ void load_packed_query(PackedTile<NB, PARTS>& t, const T* row, bool row_ok, int hd, int g) {
-  constexpr int NG = PackedTile<NB, PARTS>::NG;
-  float sum[NG] = {};
+template <int NB, bool WIDE, typename T>
+__device__ __forceinline__ void load_packed_query(PackedTile<NB, WIDE>& t, const T* row, bool row_ok, int hd, int g) {
+  constexpr int NG = PackedTile<NB, WIDE>::NG;
+  typedef T eight __attribute__((ext_vector_type(8)));
+  eight y[NB];
 #pragma unroll
   for (int s = 0; s < NB; ++s) {
-    typedef T eight __attribute__((ext_vector_type(8)));
     const int e = s * 32 + g * 8;
-    T x[8];
-    eight y = {};
-    if (row_ok && e < hd) y = *(const eight*)(row + e);
+    y[s] = eight{};
+    if (row_ok && e < hd) y[s] = *(const eight*)(row + e);
+  }
+  if constexpr (WIDE) {
+    float top = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = y[j];
-      sum[s / 2] += to_f32(x[j]);
+    for (int s = 0; s < NB; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(to_f32(y[s][j])));
+    // the largest magnitude to 2^13 .. 2^14 (a row of zeros, or of what is no number, as it is)
+    top = col4_max(top);
+    const int up = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+    t.qsum[0] = ldexpf(1.f, -max(up, -126));
+#pragma unroll
+    for (int s = 0; s < NB; ++s) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = ldexpf(to_f32(y[s][j]), max(up, -126));
+      u32x4 part[2];
+      two_parts<0>(part, x);
+      t.q[0][s] = part[0], t.q[1][s] = part[1];
     }
-    bf16x8 part[PARTS];
-    split_parts<PARTS, T>(part, x);
+  } else {
+    float sum[NG] = {};
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) t.q[p][s] = part[p];
+    for (int s = 0; s < NB; ++s) {
+      t.q[0][s] = __builtin_bit_cast(u32x4, y[s]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[s / 2] += to_f32(y[s][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) t.qsum[i] = col4_sum(sum[i]);
   }
 #pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    t.qsum[i] = col4_sum(sum[i]);
-    t.oz[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int i = 0; i < (WIDE ? 2 * NB : NG); ++i) t.oz[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int db = 0; db < 2 * NB; ++db) t.o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
   t.m = -INFINITY;
@@ -211,10 +227,10 @@ __device__ __forceinline__ void load_packed_query(PackedTile<NB, PARTS>& t, cons
 
 // Scores of 32 keys, masked softmax update, and O^T += V^T P^T.  `interior` (wave-uniform): every key is visible
 // to every row.
-template <int NB, int PARTS, bool EXTRA>
-__device__ __forceinline__ void packed_update(PackedTile<NB, PARTS>& t, const PackedBlock<NB>& b, int kb,
+template <int NB, bool WIDE, bool EXTRA>
+__device__ __forceinline__ void packed_update(PackedTile<NB, WIDE>& t, const PackedBlock<NB>& b, int kb,
                                               float scale_log2, bool interior, int g, const ScoreExtraLog2* x) {
-  constexpr int NG = PackedTile<NB, PARTS>::NG;
+  constexpr int NG = PackedTile<NB, WIDE>::NG;
   f32x4 st[2];
 #pragma unroll
   for (int blk = 0; blk < 2; ++blk) {
@@ -222,23 +238,34 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, PARTS>& t, const Pa
     for (int i = 0; i < NG; ++i) {
       const u32x4 scale = packed_scale_of<PackedBlock<NB>::G>(b.ks[blk], i);
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (PARTS == 1) {
+      if constexpr (!WIDE) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] = half_times(half_of(scale, 4 + j), t.qsum[i]);
       }
 #pragma unroll
       for (int s = 2 * i; s < 2 * i + 2 && s < NB; ++s) {
         unsigned c[4];
-        if constexpr (PARTS == 1) packed_codes<false>(b.k[blk][s], c);
-        else whole_keys(b.k[blk][s], __builtin_bit_cast(_Float16, b.kz[blk][i]), c);
-        const bf16x8 k = as_bf16x8(c[0], c[1], c[2], c[3]);
-#pragma unroll
-        for (int p = PARTS - 1; p >= 0; --p) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, t.q[p][s], acc, 0, 0, 0);
+        if constexpr (!WIDE) {
+          packed_codes<false>(b.k[blk][s], c);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(c[0], c[1], c[2], c[3]),
+                                                        __builtin_bit_cast(bf16x8, t.q[0][s]), acc, 0, 0, 0);
+        } else {
+          whole_keys(b.k[blk][s], b.kz[blk][i], c);
+          const f16x8 k = as_f16x8(c[0], c[1], c[2], c[3]);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(f16x8, t.q[1][s]), acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(f16x8, t.q[0][s]), acc, 0, 0, 0);
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         st[blk][j] = fmaf((float)half_of(scale, j), acc[j], i == 0 ? 0.f : st[blk][j]);
     }
+  }
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) st[blk][j] *= t.qsum[0];
   }
   if constexpr (EXTRA) {
 #pragma unroll
@@ -275,17 +302,15 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, PARTS>& t, const Pa
     for (int db = 0; db < 2 * NB; ++db)
 #pragma unroll
       for (int j = 0; j < 4; ++j) t.o[db][j] *= corr;
-    if constexpr (PARTS == 1) {
 #pragma unroll
-      for (int i = 0; i < NG; ++i)
+    for (int i = 0; i < (WIDE ? 2 * NB : NG); ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) t.oz[i][j] *= corr;
-    }
+      for (int j = 0; j < 4; ++j) t.oz[i][j] *= corr;
   }
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const u32x4 s0 = packed_scale_of<PackedBlock<NB>::G>(b.vs[0], i), s1 = packed_scale_of<PackedBlock<NB>::G>(b.vs[1], i);
-    if constexpr (PARTS == 1) {
+    if constexpr (!WIDE) {
       // (a multiplication and its rounding to float16 are one instruction)
       f16x8 w;
 #pragma unroll
@@ -303,35 +328,36 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, PARTS>& t, const Pa
       float w[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = half_times(half_of(j < 4 ? s0 : s1, j % 4), p[j]);
-      bf16x8 part[PARTS];
-      split_parts<PARTS, float>(part, w);
+      u32x4 part[2];
+      two_parts<11>(part, w);
+      const f16x8 hi = __builtin_bit_cast(f16x8, part[0]), lo = __builtin_bit_cast(f16x8, part[1]);
 #pragma unroll
       for (int s = 2 * i; s < 2 * i + 2 && s < NB; ++s) {
         unsigned c[4], d[4];
         whole_values(b.v[0][s], f16x2{half_of(s0, 4), half_of(s0, 5)}, f16x2{half_of(s0, 6), half_of(s0, 7)}, c);
         whole_values(b.v[1][s], f16x2{half_of(s1, 4), half_of(s1, 5)}, f16x2{half_of(s1, 6), half_of(s1, 7)}, d);
-        const bf16x8 even = as_bf16x8(c[0], c[1], d[0], d[1]), odd = as_bf16x8(c[2], c[3], d[2], d[3]);
-#pragma unroll
-        for (int q = PARTS - 1; q >= 0; --q) {
-          t.o[2 * s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, part[q], t.o[2 * s], 0, 0, 0);
-          t.o[2 * s + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, part[q], t.o[2 * s + 1], 0, 0, 0);
-        }
+        const f16x8 even = as_f16x8(c[0], c[1], d[0], d[1]), odd = as_f16x8(c[2], c[3], d[2], d[3]);
+        t.o[2 * s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, hi, t.o[2 * s], 0, 0, 0);
+        t.oz[2 * s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, lo, t.oz[2 * s], 0, 0, 0);
+        t.o[2 * s + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, hi, t.o[2 * s + 1], 0, 0, 0);
+        t.oz[2 * s + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, lo, t.oz[2 * s + 1], 0, 0, 0);
       }
     }
   }
 }
 
-// The rows' sums with what the zeros take off.
-template <int NB, int PARTS>
-__device__ __forceinline__ void packed_finish(PackedTile<NB, PARTS>& t) {
-  if constexpr (PARTS == 1) {
+// The rows' sums with what the zeros take off, or with the second parts.
+template <int NB, bool WIDE>
+__device__ __forceinline__ void packed_finish(PackedTile<NB, WIDE>& t) {
 #pragma unroll
-    for (int db = 0; db < 2 * NB; ++db)
+  for (int db = 0; db < 2 * NB; ++db)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) t.o[db][j] += t.oz[db / 4][j];
-  }
+    for (int j = 0; j < 4; ++j) t.o[db][j] = WIDE ? fmaf(t.oz[db][j], 1.f / 2048.f, t.o[db][j]) : t.o[db][j] + t.oz[db / 4][j];
   t.l = col4_sum(t.l);
 }
+
+// Workgroups of four wavefronts that a compute unit holds, by the registers they take.
+__host__ __device__ constexpr int packed_waves(int nb, bool wide) { return nb > 4 ? (wide ? 1 : 2) : wide ? 2 : 3; }
 
 constexpr int kPackedChunk = 128;      // keys: a block for each of a workgroup's wavefronts
 
@@ -347,6 +373,19 @@ __device__ __forceinline__ PackedItem packed_item(const PackedArgs& args, int ti
   it.tok0 = args.tiles ? args.tiles[tile * 3 + 1] : tile;
   it.ntok = args.tiles ? args.tiles[tile * 3 + 2] : 1;
   it.pos_first = args.base.positions[it.tok0];                // positions are consecutive
+  it.pos_last = it.pos_first + it.ntok - 1;
+  it.walk = key_walk<32>(args.base, first_visible(args.base, it.pos_first));
+  return it;
+}
+
+// The same of a tile that is the same for the whole wavefront: its numbers by scalar loads.
+__device__ __forceinline__ PackedItem packed_item_of(const PackedArgs& args, int tile) {
+  PackedItem it{tile, tile, 1, 0, 0, KeyWalk{0, 0}};
+  if (args.tiles) {
+    const ConstTable row = (ConstTable)args.tiles + tile * 3;
+    it.entry = row[0], it.tok0 = row[1], it.ntok = row[2];
+  }
+  it.pos_first = ((ConstTable)args.base.positions)[it.tok0];
   it.pos_last = it.pos_first + it.ntok - 1;
   it.walk = key_walk<32>(args.base, first_visible(args.base, it.pos_first));
   return it;
@@ -370,13 +409,13 @@ __device__ __forceinline__ int lanes_before(int v, int lane) {
 // A workgroup's four wavefronts take every fourth block of 32 keys and merge in LDS.  An item that ends in another
 // workgroup than it began in leaves its parts in memory, two places a workgroup (the part that an earlier one began, the
 // part that a later one goes on with), and whoever comes last merges them in their order.
-template <int NB, int PARTS, bool EXTRA, typename T>
-__global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_attention_kernel(PackedArgs args) {
+template <int NB, bool WIDE, bool EXTRA, typename T>
+__global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_kernel(PackedArgs args) {
   constexpr int HD = 32 * NB, DB = 2 * NB;
   constexpr int kRow = HD + 4;                                // neighbouring rows start four banks apart
   __shared__ float s_ml[4][16][2];
   __shared__ __attribute__((aligned(16))) float s_o[4][16][kRow];
-  __shared__ unsigned s_before;
+  __shared__ unsigned s_before[2];
   const AttentionArgs& a = args.base;
   const int wave = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int r = lane % 16, g = lane / 16;
@@ -385,34 +424,43 @@ __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_att
   T* out = (T*)a.out;
 
   // this workgroup's chunks [at, end) of all, and the tile in which they begin
-  int total = 0;
-  for (int t0 = 0; t0 < args.num_tiles; t0 += kWave) {
-    const int n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).chunks() * heads : 0;
-    total += uniform(__shfl(lanes_before(n, lane), kWave - 1, kWave));
-  }
-  const int len = (total + args.workgroups - 1) / args.workgroups;
-  int at = blockIdx.x * len;
-  const int end = min(at + len, total);
-  if (at >= end) return;
-  int tile = 0, tile_at = 0;                                  // the tile, and its first chunk among all
-  for (int t0 = 0, sum = 0; t0 < args.num_tiles; t0 += kWave) {
-    const int n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).chunks() * heads : 0;
-    const int upto = sum + lanes_before(n, lane);
-    const unsigned long long here = __builtin_amdgcn_ballot_w64(upto > at);
-    if (here != 0) {
-      const int l = __builtin_ctzll(here);
-      tile = t0 + l;
-      tile_at = uniform(__shfl(upto - n, l, kWave));
-      break;
+  int at, end, len = 0, tile = 0, tile_at = 0;                // tile_at: the tile's first chunk among all
+  if (args.workgroups == 0) {
+    tile = blockIdx.x / heads;
+    const int chunks = packed_item_of(args, tile).chunks();
+    at = (blockIdx.x - tile * heads) * chunks;
+    end = at + chunks;
+  } else {
+    int total = 0;
+    for (int t0 = 0; t0 < args.num_tiles; t0 += kWave) {
+      const int n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).chunks() * heads : 0;
+      total += uniform(__shfl(lanes_before(n, lane), kWave - 1, kWave));
     }
-    sum = uniform(__shfl(upto, kWave - 1, kWave));
+    len = (total + args.workgroups - 1) / args.workgroups;
+    at = blockIdx.x * len;
+    end = min(at + len, total);
+    if (at >= end) return;
+    for (int t0 = 0, sum = 0; t0 < args.num_tiles; t0 += kWave) {
+      const int n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).chunks() * heads : 0;
+      const int upto = sum + lanes_before(n, lane);
+      const unsigned long long here = __builtin_amdgcn_ballot_w64(upto > at);
+      if (here != 0) {
+        const int l = __builtin_ctzll(here);
+        tile = t0 + l;
+        tile_at = uniform(__shfl(upto - n, l, kWave));
+        break;
+      }
+      sum = uniform(__shfl(upto, kWave - 1, kWave));
+    }
   }
+  // the parts that this workgroup leaves in memory, one that an earlier one began and one that a later one goes on with
+  struct Part {
+    int item, first_wg, parts, rows, hb, kvh, tok0;
+  } part[2];
+  int left = 0;
 
   while (at < end) {
-    PackedItem it = packed_item(args, uniform(tile));
-    it.entry = uniform(it.entry), it.tok0 = uniform(it.tok0), it.ntok = uniform(it.ntok);
-    it.pos_first = uniform(it.pos_first), it.pos_last = uniform(it.pos_last);
-    it.walk.begin = uniform(it.walk.begin), it.walk.origin = uniform(it.walk.origin);
+    const PackedItem it = packed_item_of(args, uniform(tile));
     const int chunks = it.chunks(), head_of = (at - tile_at) / chunks, first_chunk = at - tile_at - head_of * chunks;
     const int count = min(chunks - first_chunk, end - at);
     const int item_at = at - first_chunk, item = tile * heads + head_of;
@@ -430,27 +478,25 @@ __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_att
     PageCursor cur{(ConstTable)table, a.page_size, it.pos_last, it.walk, -1, -1};
     cur.start(key_begin);
     PackedBlock<NB> A, B;
-    load_packed<NB, PARTS>(A, a, cur, kvh, key_begin, kPackedChunk, lane);
-    PackedTile<NB, PARTS> t;
+    load_packed<NB, WIDE>(A, a, cur, kvh, key_begin, kPackedChunk, lane);
+    PackedTile<NB, WIDE> t;
     t.pos = row_ok ? it.pos_first + ti : -1;
     t.lo = first_visible(a, t.pos);
     t.keep = a.keep;
-    load_packed_query<NB, PARTS, T>(t, (const T*)a.q + ((int64_t)token * a.nq + head) * a.hd, row_ok, a.hd, g);
+    load_packed_query<NB, WIDE, T>(t, (const T*)a.q + ((int64_t)token * a.nq + head) * a.hd, row_ok, a.hd, g);
     ScoreExtraLog2 x;
     if (EXTRA) x = in_log2(score_extra(a, head, t.pos));
     const int lo_last = first_visible(a, it.pos_last);
     auto update = [&](const PackedBlock<NB>& b, int v) {
       const int kb = it.walk.real(v);
-      packed_update<NB, PARTS, EXTRA>(t, b, kb, scale_log2, kb + 31 <= it.pos_first && kb >= lo_last, g, &x);
+      packed_update<NB, WIDE, EXTRA>(t, b, kb, scale_log2, kb + 31 <= it.pos_first && kb >= lo_last, g, &x);
     };
-    for (int v = key_begin; v < key_end; v += 2 * kPackedChunk) {
-      load_packed<NB, PARTS>(B, a, cur, kvh, v + kPackedChunk, kPackedChunk, lane);
+    for (int v = key_begin; v < key_end; v += kPackedChunk) {
+      load_packed<NB, WIDE>(B, a, cur, kvh, v + kPackedChunk, kPackedChunk, lane);
       update(A, v);
-      if (v + kPackedChunk >= key_end) break;
-      load_packed<NB, PARTS>(A, a, cur, kvh, v + 2 * kPackedChunk, kPackedChunk, lane);
-      update(B, v + kPackedChunk);
+      A = B;
     }
-    packed_finish<NB, PARTS>(t);
+    packed_finish<NB, WIDE>(t);
 
     // the wavefronts' results through LDS, an element at a time to a thread (rows that exist only)
     if (g == 0) {
@@ -495,60 +541,67 @@ __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_att
       }
     }
     if (!whole) {
-      // The parts' results pass the caches that another XCD does not share; each wave waits until its own have
-      // been taken, the workgroup counts itself in, and the one that finds all others there merges.
-      const int first_wg = item_at / len, parts = (item_at + chunks - 1) / len - first_wg + 1;
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
-      if (threadIdx.x == 0)
-        s_before = __hip_atomic_fetch_add(args.arrivals + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __syncthreads();
-      if ((int)s_before + 1 == parts) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-        if (threadIdx.x == 0) __hip_atomic_store(args.arrivals + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        for (int e = threadIdx.x; e < rows * HD; e += 256) {
-          const int row = e / HD, d = e % HD;
-          const int64_t to = place(row);
-          if (to < 0 || d >= a.hd) continue;
-          float M = -INFINITY, sum = 0.f, acc = 0.f;
-          for (int s0 = 0; s0 < parts; s0 += 4) {             // four at a time: everything asked for before its use
-            float ms[4], ls[4], part[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int p = min(s0 + j, parts - 1);
-              const int64_t slot = ((int64_t)(first_wg + p) * 2 + (p == 0 ? 1 : 0)) * 16 + row;
-              const uint64_t ml = __hip_atomic_load((const uint64_t*)args.partial_ml + slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-              ms[j] = s0 + j < parts ? __uint_as_float((unsigned)ml) : -INFINITY;
-              ls[j] = __uint_as_float((unsigned)(ml >> 32));
-              part[j] = __hip_atomic_load(args.partial_o + slot * HD + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-            float Mg = M;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) Mg = fmaxf(Mg, ms[j]);
-            const float Mc = Mg == -INFINITY ? 0.f : Mg, keep = __builtin_amdgcn_exp2f(M - Mc);
-            sum *= keep;
-            acc *= keep;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float w = __builtin_amdgcn_exp2f(ms[j] - Mc);
-              sum = fmaf(ls[j], w, sum);
-              acc = fmaf(part[j], w, acc);
-            }
-            M = Mg;
-          }
-          sum = sum_with_sink(sum, M, a.sink, sink_of(row));
-          out[to + d] = from_f32<T>(acc * (sum > 0.f ? 1.f / sum : 0.f));
-        }
-      }
+      const int first_wg = item_at / len;
+      part[left > 0 ? 1 : 0] = Part{item, first_wg, (item_at + chunks - 1) / len - first_wg + 1, rows, hb, kvh, it.tok0};
+      ++left;
     }
     if (at < end) __syncthreads();                            // everybody has read what stands in LDS
+  }
+  if (left == 0) return;
+
+  // The parts' results pass the caches that another XCD does not share; each wave waits until its own have
+  // been taken, the workgroup counts itself in for both, and the one that finds all others there merges.
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if ((int)threadIdx.x < left)
+    s_before[threadIdx.x] = __hip_atomic_fetch_add(args.arrivals + (threadIdx.x == 0 ? part[0].item : part[1].item), 1u,
+                                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  for (int which = 0; which < left; ++which) {
+    const Part p = which == 0 ? part[0] : part[1];
+    if ((int)s_before[which] + 1 != p.parts) continue;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    if (threadIdx.x == 0) __hip_atomic_store(args.arrivals + p.item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int e = threadIdx.x; e < p.rows * HD; e += 256) {
+      const int row = e / HD, d = e % HD;
+      const int rt = row / args.rows_per_token, rh = p.hb * 16 + row % args.rows_per_token;
+      if (rh >= group || d >= a.hd) continue;
+      float M = -INFINITY, sum = 0.f, acc = 0.f;
+      for (int s0 = 0; s0 < p.parts; s0 += 4) {               // four at a time: everything asked for before its use
+        float ms[4], ls[4], po[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int n = min(s0 + j, p.parts - 1);
+          const int64_t slot = ((int64_t)(p.first_wg + n) * 2 + (n == 0 ? 1 : 0)) * 16 + row;
+          const uint64_t ml = __hip_atomic_load((const uint64_t*)args.partial_ml + slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          ms[j] = s0 + j < p.parts ? __uint_as_float((unsigned)ml) : -INFINITY;
+          ls[j] = __uint_as_float((unsigned)(ml >> 32));
+          po[j] = __hip_atomic_load(args.partial_o + slot * HD + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        float Mg = M;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Mg = fmaxf(Mg, ms[j]);
+        const float Mc = Mg == -INFINITY ? 0.f : Mg, keep = __builtin_amdgcn_exp2f(M - Mc);
+        sum *= keep;
+        acc *= keep;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float w = __builtin_amdgcn_exp2f(ms[j] - Mc);
+          sum = fmaf(ls[j], w, sum);
+          acc = fmaf(po[j], w, acc);
+        }
+        M = Mg;
+      }
+      sum = sum_with_sink(sum, M, a.sink, p.kvh * group + rh);
+      out[((int64_t)(p.tok0 + rt) * a.nq + p.kvh * group + rh) * a.hd + d] = from_f32<T>(acc * (sum > 0.f ? 1.f / sum : 0.f));
+    }
   }
 }
 
 // A wavefront per tile and head, which walks its keys alone: tiles enough to fill the chip (prompts).
-template <int NB, int PARTS, bool EXTRA, typename T>
-__global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_walk_kernel(PackedArgs args) {
+template <int NB, bool WIDE, bool EXTRA, typename T>
+__global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_walk_kernel(PackedArgs args) {
   constexpr int DB = 2 * NB;
   const AttentionArgs& a = args.base;
   const int wave = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
@@ -557,10 +610,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_wal
   const int item = blockIdx.x * 4 + wave;
   if (item >= args.num_tiles * heads) return;
   const int hb = item % args.head_blocks, kvh = item / args.head_blocks % a.nkv;
-  PackedItem it = packed_item(args, uniform(item / heads));
-  it.entry = uniform(it.entry), it.tok0 = uniform(it.tok0), it.ntok = uniform(it.ntok);
-  it.pos_first = uniform(it.pos_first), it.pos_last = uniform(it.pos_last);
-  it.walk.begin = uniform(it.walk.begin), it.walk.origin = uniform(it.walk.origin);
+  const PackedItem it = packed_item_of(args, uniform(item / heads));
   const int ti = r / args.rows_per_token, hh = hb * 16 + r % args.rows_per_token;
   const bool row_ok = ti < it.ntok && hh < group;
   const int token = it.tok0 + min(ti, it.ntok - 1), head = kvh * group + min(hh, group - 1);
@@ -568,28 +618,26 @@ __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_wal
   PageCursor cur{(ConstTable)(a.table + (int64_t)it.entry * a.table_width), a.page_size, it.pos_last, it.walk, -1, -1};
   cur.start(key_begin);
   PackedBlock<NB> A, B;
-  load_packed<NB, PARTS>(A, a, cur, kvh, key_begin, 32, lane);
-  PackedTile<NB, PARTS> t;
+  load_packed<NB, WIDE>(A, a, cur, kvh, key_begin, 32, lane);
+  PackedTile<NB, WIDE> t;
   t.pos = row_ok ? it.pos_first + ti : -1;
   t.lo = first_visible(a, t.pos);
   t.keep = a.keep;
-  load_packed_query<NB, PARTS, T>(t, (const T*)a.q + ((int64_t)token * a.nq + head) * a.hd, row_ok, a.hd, g);
+  load_packed_query<NB, WIDE, T>(t, (const T*)a.q + ((int64_t)token * a.nq + head) * a.hd, row_ok, a.hd, g);
   ScoreExtraLog2 x;
   if (EXTRA) x = in_log2(score_extra(a, head, t.pos));
   const int lo_last = first_visible(a, it.pos_last);
   auto update = [&](const PackedBlock<NB>& b, int v) {
     const int kb = it.walk.real(v);
-    packed_update<NB, PARTS, EXTRA>(t, b, kb, a.scale * 1.44269504088896341f,
+    packed_update<NB, WIDE, EXTRA>(t, b, kb, a.scale * 1.44269504088896341f,
                                     kb + 31 <= it.pos_first && kb >= lo_last, g, &x);
   };
-  for (int v = key_begin; v < key_end; v += 64) {
-    load_packed<NB, PARTS>(B, a, cur, kvh, v + 32, 32, lane);
+  for (int v = key_begin; v < key_end; v += 32) {
+    load_packed<NB, WIDE>(B, a, cur, kvh, v + 32, 32, lane);
     update(A, v);
-    if (v + 32 >= key_end) break;
-    load_packed<NB, PARTS>(A, a, cur, kvh, v + 64, 32, lane);
-    update(B, v + 32);
+    A = B;
   }
-  packed_finish<NB, PARTS>(t);
+  packed_finish<NB, WIDE>(t);
   if (!row_ok) return;
   const float sum = sum_with_sink(t.l, t.m, a.sink, head), inv = sum > 0.f ? 1.f / sum : 0.f;
   typedef T four __attribute__((ext_vector_type(4)));
@@ -603,28 +651,28 @@ __global__ __launch_bounds__(256, PARTS == 1 && NB <= 4 ? 2 : 1) void packed_wal
   }
 }
 
-template <int NB, int PARTS, bool EXTRA, typename T>
+template <int NB, bool WIDE, bool EXTRA, typename T>
 static int launch_packed(const PackedArgs& args, bool coop, hipStream_t stream) {
   const int items = args.num_tiles * args.base.nkv * args.head_blocks;
   if (coop)
-    hipLaunchKernelGGL((packed_attention_kernel<NB, PARTS, EXTRA, T>), dim3(args.workgroups), dim3(256), 0, stream, args);
+    hipLaunchKernelGGL((packed_attention_kernel<NB, WIDE, EXTRA, T>), dim3(args.workgroups ? args.workgroups : items), dim3(256), 0, stream, args);
   else
-    hipLaunchKernelGGL((packed_walk_kernel<NB, PARTS, EXTRA, T>), dim3((items + 3) / 4), dim3(256), 0, stream, args);
+    hipLaunchKernelGGL((packed_walk_kernel<NB, WIDE, EXTRA, T>), dim3((items + 3) / 4), dim3(256), 0, stream, args);
   TS_CHECK_LAUNCH("packed_attention");
   return 0;
 }
 
 // A translation unit's heads: of so many slices of 32 elements.
-#define TS_PACKED_CASES(PARTS, EXTRA, T)                                      \
+#define TS_PACKED_CASES(WIDE, EXTRA, T)                                      \
   switch (pack_slices(args.base.hd)) {                                        \
-    case 1: return launch_packed<1, PARTS, EXTRA, T>(args, coop, stream);     \
-    case 2: return launch_packed<2, PARTS, EXTRA, T>(args, coop, stream);     \
-    case 3: return launch_packed<3, PARTS, EXTRA, T>(args, coop, stream);     \
-    case 4: return launch_packed<4, PARTS, EXTRA, T>(args, coop, stream);     \
-    case 5: return launch_packed<5, PARTS, EXTRA, T>(args, coop, stream);     \
-    case 6: return launch_packed<6, PARTS, EXTRA, T>(args, coop, stream);     \
-    case 7: return launch_packed<7, PARTS, EXTRA, T>(args, coop, stream);     \
-    case 8: return launch_packed<8, PARTS, EXTRA, T>(args, coop, stream);     \
+    case 1: return launch_packed<1, WIDE, EXTRA, T>(args, coop, stream);     \
+    case 2: return launch_packed<2, WIDE, EXTRA, T>(args, coop, stream);     \
+    case 3: return launch_packed<3, WIDE, EXTRA, T>(args, coop, stream);     \
+    case 4: return launch_packed<4, WIDE, EXTRA, T>(args, coop, stream);     \
+    case 5: return launch_packed<5, WIDE, EXTRA, T>(args, coop, stream);     \
+    case 6: return launch_packed<6, WIDE, EXTRA, T>(args, coop, stream);     \
+    case 7: return launch_packed<7, WIDE, EXTRA, T>(args, coop, stream);     \
+    case 8: return launch_packed<8, WIDE, EXTRA, T>(args, coop, stream);     \
   }                                                                           \
   TS_FAIL("packed_attention: head_dim=%d not built", args.base.hd)
 

@@ -156,6 +156,8 @@ class Dispatch:
     # time; `packed_workgroups` another number), above it a wavefront walks a tile's keys.
     packed_items: int = 2048
     packed_workgroups: int = 0
+    #: up to so many chunks of 128 keys an item is one workgroup's
+    packed_whole: int = 8
 
     # ---- recurrences.  A step whose longest portion has more tokens than this runs in chunks of
     # 64 tokens as products of matrices, below it every entry is walked whole by one launch.

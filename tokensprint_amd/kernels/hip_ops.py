@@ -1196,14 +1196,16 @@ class HipOps:
         d = self.dispatch
         coop = items <= d.packed_items
         if coop:
-            # a workgroup for every 128 keys that there can be, as many as the card holds at a time
-            m.workgroups = min(items * -(-keys // 128),
-                               d.packed_workgroups or self.lib.ts_packed_resident(a.hd, _TYPE_CODE[dtype]))
-            hd = -(-a.hd // 32) * 32
-            partial = torch.empty(m.workgroups * 32 * (hd + 2), dtype=torch.float32, device=self.device)
-            m.partial_o = partial.data_ptr()
-            m.partial_ml = m.partial_o + m.workgroups * 32 * hd * 4
-            m.arrivals = self._counts(items).data_ptr()
+            chunks = -(-keys // 128)
+            if chunks > d.packed_whole:
+                # a workgroup for every 128 keys that there can be, as many as the card holds at a time
+                m.workgroups = min(items * chunks, d.packed_workgroups
+                                   or self.lib.ts_packed_resident(a.hd, _TYPE_CODE[dtype]))
+                hd = -(-a.hd // 32) * 32
+                partial = torch.empty(m.workgroups * 32 * (hd + 2), dtype=torch.float32, device=self.device)
+                m.partial_o = partial.data_ptr()
+                m.partial_ml = m.partial_o + m.workgroups * 32 * hd * 4
+                m.arrivals = self._counts(items).data_ptr()
         self._call(self.lib.ts_packed_attention, byref(m), _TYPE_CODE[dtype], int(coop), self._stream())
 
     def attend(self, qkv, batch, table, cache, write_cache, *, num_heads, num_kv_heads,
