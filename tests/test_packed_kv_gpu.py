@@ -267,6 +267,39 @@ def check_attention(ops, device, *, nq, nkv, hd, page, spans, dtype, seed=0, **o
     return got
 
 
+LONG = {"one": [(0, 700)], "behind": [(333, 400), (0, 65), (1, 16)], "beside": [(600, 1), (40, 129), (3, 1), (0, 300), (900, 2)]}
+
+
+@pytest.mark.parametrize("spans", list(LONG))
+@pytest.mark.parametrize("nq,nkv,hd,page", [(8, 4, 128, 16), (4, 1, 64, 32), (6, 2, 128, 64), (20, 1, 64, 16), (3, 3, 128, 256),
+                                            (4, 2, 96, 16)])
+@pytest.mark.parametrize("window", [None, 100])
+def test_portions_of_prompts(ops, gpu_device, spans, nq, nkv, hd, page, window):
+    check_attention(ops, gpu_device, nq=nq, nkv=nkv, hd=hd, page=page, spans=LONG[spans], dtype=torch.bfloat16,
+                    window=window)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-4, 1e4, 1e30])
+def test_queries_of_any_magnitude(ops, gpu_device, scale):
+    """A row of queries is brought to float16's range: whatever it was, and rows of zeros."""
+    nq, nkv, hd = 4, 2, 64
+    batch, whole, table, cache = scene(gpu_device, nkv=nkv, hd=hd, page=16, spans=[(30, 40), (50, 1)])
+    k, v = heads_of(whole, nkv, hd, torch.bfloat16, gpu_device, 3)
+    ops.kv_store(k, v, whole, table, cache)
+    q = rand((41, nq, hd), torch.float32, gpu_device, 4)
+    q[7] = 0
+    q[:, :, 5] *= 1e-3
+    for dtype in DTYPES:
+        x = (q * scale).to(dtype)
+        got = ops.paged_attention(x, batch, table, cache, num_heads=nq, num_kv_heads=nkv, head_dim=hd,
+                                  scale=float(0.125 / scale), window=None)
+        want, size = attention(x, by_entry(quantize4(k), whole), by_entry(quantize4(v), whole), batch,
+                               num_kv_heads=nkv, scale=float(0.125 / scale))
+        # as in check_attention, float32's bound without the sums' share
+        bound = (2.0 ** -8 * (size + want.abs()) if dtype == torch.bfloat16 else 0) + 1e-4 * size + 1e-5
+        assert bool(((got.double().cpu() - want).abs() <= bound).all())
+
+
 SPANS = {
     "one key": [(0, 1)],
     "decode": [(40, 1), (0, 1), (255, 1), (126, 1), (31, 1), (300, 1)],
@@ -295,9 +328,9 @@ OPTIONS = {
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("spans", ["decode", "mixed"])
 @pytest.mark.parametrize("options", list(OPTIONS))
-@pytest.mark.parametrize("walk", ["shares", "one workgroup", "whole items", "wavefronts"])
+@pytest.mark.parametrize("walk", ["shares", "one workgroup", "whole items", "wavefronts", "portions"])
 def test_attention_options(ops, gpu_device, dispatch, dtype, spans, options, walk):
-    dispatch(packed_items=0 if walk == "wavefronts" else 1 << 20, packed_whole=1 << 20 if walk == "whole items" else 0,
+    dispatch(packed_portion=1 if walk == "portions" else 1 << 20, packed_items=0 if walk == "wavefronts" else 1 << 20, packed_whole=1 << 20 if walk == "whole items" else 0,
              packed_workgroups={"shares": 0, "one workgroup": 1}.get(walk, 7))
     kw = dict(OPTIONS[options])
     nq, nkv, hd = 6, 2, 64

@@ -151,13 +151,15 @@ class Dispatch:
     cooperative_workgroups: int = 512
     per_wave_workgroups: int = 4096
 
-    # ---- attention over keys and values of 4 bits: up to so many tiles of 16 rows (times key/value
-    # heads) all their keys are shared out evenly over workgroups (as many as the card holds at a
-    # time; `packed_workgroups` another number), above it a wavefront walks a tile's keys.
+    # ---- attention over keys and values of 4 bits: portions of at least `packed_portion` tokens have
+    # the kernel that makes tiles in LDS; of tiles of 16 rows (times key/value heads), up to
+    # `packed_items` have all their keys shared out evenly over workgroups (as many as the card holds at
+    # a time; `packed_workgroups` another number), more a wavefront each; up to so many chunks of 128
+    # keys an item is one workgroup's.
+    packed_portion: int = 16
     packed_items: int = 2048
     packed_workgroups: int = 0
-    #: up to so many chunks of 128 keys an item is one workgroup's
-    packed_whole: int = 8
+    packed_whole: int = 10
 
     # ---- recurrences.  A step whose longest portion has more tokens than this runs in chunks of
     # 64 tokens as products of matrices, below it every entry is walked whole by one launch.

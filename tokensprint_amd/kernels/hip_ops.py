@@ -1177,36 +1177,61 @@ class HipOps:
         return out
 
     def _attention_packed(self, a, batch, group, dtype):
-        """Attention over a cache of 4 bits: tiles of 16 rows (query heads of a key/value head x
-        tokens); few tiles have a workgroup each and share of their keys, many a wavefront
-        each."""
+        """Attention over a cache of 4 bits: portions of prompts by the kernel that makes tiles in LDS
+        (bfloat16, heads of 64 and 128), everything else in tiles of 16 rows (query heads of a key/value
+        head x tokens), whose keys are shared out over workgroups where the tiles are few."""
         if not a.scale > 0:
             raise ValueError(f"attention over keys of 4 bits: scale={a.scale} must be positive")
-        m = PackedArgs()
-        m.base = a
-        m.rows_per_token, m.head_blocks = min(group, 16), -(-group // 16)
-        if batch.max_q_len == 1:
-            m.num_tiles = batch.num_entries
-        else:
-            tiles, m.num_tiles = self._attention_tiles(batch, 16 // m.rows_per_token)
-            m.tiles = tiles.data_ptr()
-        items = m.num_tiles * a.nkv * m.head_blocks
-        reach = self._reach(a)
-        keys = batch.max_ctx_len if reach == 0 else min(batch.max_ctx_len, reach + batch.max_q_len + 64)
-        d = self.dispatch
-        coop = items <= d.packed_items
-        if coop:
-            chunks = -(-keys // 128)
-            if chunks > d.packed_whole:
-                # a workgroup for every 128 keys that there can be, as many as the card holds at a time
-                m.workgroups = min(items * chunks, d.packed_workgroups
-                                   or self.lib.ts_packed_resident(a.hd, _TYPE_CODE[dtype]))
-                hd = -(-a.hd // 32) * 32
-                partial = torch.empty(m.workgroups * 32 * (hd + 2), dtype=torch.float32, device=self.device)
-                m.partial_o = partial.data_ptr()
-                m.partial_ml = m.partial_o + m.workgroups * 32 * hd * 4
-                m.arrivals = self._counts(items).data_ptr()
-        self._call(self.lib.ts_packed_attention, byref(m), _TYPE_CODE[dtype], int(coop), self._stream())
+        d, tokens = self.dispatch, 16 // min(group, 16)
+        tall = dtype is torch.bfloat16 and self.lib.ts_packed_prompt_fits(a.hd) == 1
+        for portions in (True, False):
+            count, tiles = self._packed_tiles(batch, portions, 8 * tokens if portions and tall else tokens,
+                                              d.packed_portion)
+            if count == 0:
+                continue
+            m = PackedArgs()
+            m.base = a
+            m.rows_per_token, m.head_blocks = min(group, 16), -(-group // 16)
+            m.num_tiles, m.tiles = count, tiles
+            items = count * a.nkv * m.head_blocks
+            if portions and tall:
+                # two sets of wavefronts share an item's keys where items leave units empty
+                self._call(self.lib.ts_packed_prompt, byref(m), 2 if items <= self._units else 1, self._stream())
+                continue
+            shared = items <= d.packed_items
+            if shared:
+                reach = self._reach(a)
+                keys = batch.max_ctx_len if reach == 0 else min(batch.max_ctx_len, reach + batch.max_q_len + 64)
+                chunks = -(-keys // 128)
+                if chunks > d.packed_whole:
+                    # a workgroup for every 128 keys that there can be, as many as the card holds at a time
+                    m.workgroups = min(items * chunks, d.packed_workgroups
+                                       or self.lib.ts_packed_resident(a.hd, _TYPE_CODE[dtype]))
+                    hd = -(-a.hd // 32) * 32
+                    partial = torch.empty(m.workgroups * 32 * (hd + 2), dtype=torch.float32, device=self.device)
+                    m.partial_o = partial.data_ptr()
+                    m.partial_ml = m.partial_o + m.workgroups * 32 * hd * 4
+                    m.arrivals = self._counts(items).data_ptr()
+            self._call(self.lib.ts_packed_attention, byref(m), _TYPE_CODE[dtype], int(shared), self._stream())
+
+    def _packed_tiles(self, batch, portions, tokens, least):
+        """(number, device address or None) of the runs of at most `tokens` consecutive tokens of the
+        batch's entries that bring at least `least` tokens (`portions`), or of the others; those that see
+        most keys first.  A step of single tokens needs no list."""
+        if batch.max_q_len == 1 and batch.num_tokens == batch.num_entries:
+            return (0, None) if portions else (batch.num_entries, None)
+        key = ("packed_tiles", portions, tokens, least)
+        if key not in batch.plans:
+            tiles, first = [], 0
+            for entry, (n, start) in enumerate(zip(batch.q_lens, batch.starts)):
+                if (n >= least) == portions:
+                    tiles += [(start + min(t0 + tokens, n), entry, first + t0, min(tokens, n - t0))
+                              for t0 in range(0, n, tokens)]
+                first += n
+            tiles.sort(key=lambda t: -t[0])
+            batch.plans[key] = (self._upload_ints([t[1:] for t in tiles]) if tiles else None, len(tiles))
+        held, count = batch.plans[key]
+        return count, held.data_ptr() if count else None
 
     def attend(self, qkv, batch, table, cache, write_cache, *, num_heads, num_kv_heads,
                kv_in_row, head_dim, q_weight, k_weight, eps, cos_sin, scale, window,
