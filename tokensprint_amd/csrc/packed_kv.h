@@ -32,6 +32,8 @@
 // element j = 2 p of keys for p < 4, 2 (p - 4) + 1 else; of values, token i of the first element for p = i / 2 + 4
 // (i % 2), of the second 2 further.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 constexpr int kPackGroup = 64;     // elements
@@ -63,28 +65,51 @@ struct PackGroup {
 };
 
 // The group of the eight lanes that hold 64 elements between them, eight each (`v`; elements that are not there are
-// zeros), and this lane's codes.
+// zeros), and this lane's codes.  A quotient by the estimate of 1 / step is off by less than 2^-18, so a code is the whole
+// number next to it unless that is nearly half a step away; where one of a wavefront's is, all are worked out with what is
+// left over (exactly: ties to even), and where one is no finite number, they are made one.
 __device__ __forceinline__ PackGroup pack_eight(float (&v)[8], unsigned (&code)[8]) {
   constexpr float kMost = 3.4028234663852886e38f;
-  float lo = 0.f, hi = 0.f;
+  float none = 0.f;                                            // NaN if an element is not finite
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    v[j] = v[j] == v[j] ? fminf(fmaxf(v[j], -kMost), kMost) : 0.f;
-    lo = fminf(lo, v[j]);
-    hi = fmaxf(hi, v[j]);
-  }
+  for (int j = 0; j < 8; ++j) none = fmaf(v[j], 0.f, none);
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(none != none) != 0, 0)) {
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, o, kWave));
-    hi = fmaxf(hi, __shfl_xor(hi, o, kWave));
+    for (int j = 0; j < 8; ++j) v[j] = v[j] == v[j] ? fminf(fmaxf(v[j], -kMost), kMost) : 0.f;
   }
+  float lo = fminf(fminf(v[0], v[1]), 0.f), hi = fmaxf(fmaxf(v[0], v[1]), 0.f);
+#pragma unroll
+  for (int j = 2; j < 8; j += 2) {
+    lo = fminf(fminf(lo, v[j]), v[j + 1]);
+    hi = fmaxf(fmaxf(hi, v[j]), v[j + 1]);
+  }
+  // (the neighbour's, the other pair's, then the other four's: lane moves, not trips through LDS)
+  auto from = [](float x, auto how) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(how)::value, 0xf, 0xf, true));
+  };
+  lo = fminf(lo, from(lo, std::integral_constant<int, 0xB1>{})), hi = fmaxf(hi, from(hi, std::integral_constant<int, 0xB1>{}));
+  lo = fminf(lo, from(lo, std::integral_constant<int, 0x4E>{})), hi = fmaxf(hi, from(hi, std::integral_constant<int, 0x4E>{}));
+  lo = fminf(lo, from(lo, std::integral_constant<int, 0x141>{})), hi = fmaxf(hi, from(hi, std::integral_constant<int, 0x141>{}));
   PackGroup p;
   p.step = (_Float16)fminf((hi - lo) / 15.f, 65504.f);
-  const float step = (float)p.step, inv = step > 0.f ? 1.f / step : 0.f;
-  p.zero = step > 0.f ? fminf(nearest_whole(-lo, step, inv), 15.f) : 0.f;
+  const float step = (float)p.step, inv = step > 0.f ? __builtin_amdgcn_rcpf(step) : 0.f;
+  float c[8], off;
+  p.zero = rintf(-lo * inv);
+  off = fabsf(fmaf(-lo, inv, -p.zero));
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    code[j] = step > 0.f ? (unsigned)fminf(fmaxf(nearest_whole(v[j], step, inv) + p.zero, 0.f), 15.f) : 0u;
+  for (int j = 0; j < 8; ++j) {
+    const float x = v[j] * inv;
+    c[j] = rintf(x);
+    off = fmaxf(off, fabsf(x - c[j]));
+  }
+  if (__builtin_amdgcn_ballot_w64(off > 0.4999f || step >= 65504.f) != 0) {
+    p.zero = nearest_whole(-lo, step, inv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = nearest_whole(v[j], step, inv);
+  }
+  p.zero = step > 0.f ? fminf(p.zero, 15.f) : 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) code[j] = (unsigned)__builtin_amdgcn_fmed3f(c[j] + p.zero, 0.f, 15.f);
   return p;
 }
 

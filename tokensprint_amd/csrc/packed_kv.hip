@@ -18,6 +18,7 @@ struct PackStoreArgs {
   int64_t stride;            // elements from a token's row to the next, the same in q, k and v
   int table_width, num_tokens, nq, nkv, hd, page_size;
   float eps;
+  unsigned heads, heads_inv;     // heads of a token's row (inverse32: common.h)
 };
 
 // LANES: of a head (8, 16, 32), eight elements each.
@@ -25,10 +26,9 @@ template <typename T, int LANES>
 __global__ __launch_bounds__(256) void pack_store_kernel(PackStoreArgs a) {
   constexpr int kHeads = kWave / LANES;
   const int lane = threadIdx.x % kWave, sub = lane % LANES;
-  const int heads = a.nq + 2 * a.nkv;
-  const int64_t item = ((int64_t)blockIdx.x * 4 + threadIdx.x / kWave) * kHeads + lane / LANES;
-  if (item >= (int64_t)a.num_tokens * heads) return;          // whole heads: groups of LANES lanes
-  const int t = (int)(item / heads), h = (int)(item - (int64_t)t * heads);
+  const unsigned item = (blockIdx.x * 4 + threadIdx.x / kWave) * kHeads + lane / LANES;
+  const int t = (int)divided(item, a.heads, a.heads_inv), h = (int)(item - t * a.heads);
+  if (t >= a.num_tokens) return;                               // whole heads: groups of LANES lanes
   const int hd = a.hd, pos = a.positions[t], entry = a.entry_of_token[t];
   const bool there = sub * 8 < hd;
   const int at = there ? sub * 8 : 0;
@@ -71,13 +71,13 @@ __global__ __launch_bounds__(256) void pack_store_kernel(PackStoreArgs a) {
       }
       return;
     }
-    const int page = a.table[(int64_t)entry * a.table_width + pos / a.page_size];
+    const int page = a.table[(int64_t)entry * a.table_width + (pos >> __builtin_ctz(a.page_size))];
     unsigned code[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = there ? to_f32(from_f32<T>(v[j])) : 0.f;
     const PackGroup p = pack_eight(v, code);
     if (page < 0) return;                                      // no page behind this position: nothing is written
-    const int slot = pos % a.page_size, token = slot % kPackTokens;
+    const int slot = pos & (a.page_size - 1), token = slot % kPackTokens;
     unsigned char* block = a.k_pages + pack_block(page, a.nkv, head, a.page_size, slot, bytes);
     unsigned word = 0;
 #pragma unroll
@@ -100,8 +100,8 @@ __global__ __launch_bounds__(256) void pack_store_kernel(PackStoreArgs a) {
     if (count == j && i0 + j < 4 && t + j < a.num_tokens && a.entry_of_token[n] == entry && a.positions[n] == pos + j)
       count = j + 1;
   }
-  const int page = a.table[(int64_t)entry * a.table_width + pos / a.page_size];
-  const int slot = pos % a.page_size, quad = slot % kPackTokens / 4, second = sub / 2 % 2;
+  const int page = a.table[(int64_t)entry * a.table_width + (pos >> __builtin_ctz(a.page_size))];
+  const int slot = pos & (a.page_size - 1), quad = slot % kPackTokens / 4, second = sub / 2 % 2;
   Eight<T> x[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -157,12 +157,13 @@ __global__ __launch_bounds__(256) void pack_store_kernel(PackStoreArgs a) {
   }
 }
 
-static int launch_pack_store(const PackStoreArgs& a, int type, hipStream_t stream) {
+static int launch_pack_store(PackStoreArgs a, int type, hipStream_t stream) {
   const int lanes = a.hd <= 64 ? 8 : a.hd <= 128 ? 16 : 32;
-  const int64_t items = (int64_t)a.num_tokens * (a.nq + 2 * a.nkv);
+  a.heads = a.nq + 2 * a.nkv, a.heads_inv = inverse32(a.heads);
+  const int64_t items = (int64_t)a.num_tokens * a.heads;
   const int per_block = 4 * (kWave / lanes);
   const int64_t blocks = (items + per_block - 1) / per_block;
-  if (blocks > 2147483647LL) TS_FAIL("pack_store: too many tokens");
+  if (items > 2147483647LL - per_block) TS_FAIL("pack_store: too many tokens");
 #define TS_LAUNCH(L) hipLaunchKernelGGL((pack_store_kernel<T, L>), dim3((unsigned)blocks), dim3(256), 0, stream, a)
   TS_DISPATCH_TYPE(type, T, if (lanes == 8) TS_LAUNCH(8); else if (lanes == 16) TS_LAUNCH(16); else TS_LAUNCH(32));
 #undef TS_LAUNCH
@@ -218,50 +219,64 @@ extern "C" int ts_pack_store(const void* k, const void* v, int type, void* k_pag
 }
 
 // ---------------------------------------------------------------- back out of the cache
-// Eight elements a lane, an item a token's key or value head; positions without a page read as zeros.
+// Eight elements a lane of a token's key or value head; the first of up to four tokens that share words of values reads
+// for all of them.  Positions without a page read as zeros.
+struct PackValuesArgs {
+  const unsigned char *k_pages, *v_pages;
+  void *k, *v;                   // [T, nkv, hd]
+  const int *positions, *entry_of_token, *table;
+  int table_width, num_tokens, nkv, hd, page_size;
+  unsigned per, per_inv, heads_inv;      // pieces of a head; of 2 nkv
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void pack_values_kernel(const unsigned char* __restrict__ k_pages,
-                                                          const unsigned char* __restrict__ v_pages,
-                                                          T* __restrict__ k, T* __restrict__ v,
-                                                          const int* __restrict__ positions,
-                                                          const int* __restrict__ entry_of_token,
-                                                          const int* __restrict__ table, int table_width,
-                                                          int64_t pieces, int nkv, int hd, int page_size) {
-  const int64_t piece = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (piece >= pieces) return;
-  const int per = hd / 8, sub = (int)(piece % per);
-  const int64_t row = piece / per;                             // of [T, 2, nkv]
-  const int t = (int)(row / (2 * nkv)), h = (int)(row % (2 * nkv));
-  const bool key = h < nkv;
-  const int head = key ? h : h - nkv, pos = positions[t];
-  const int page = table[(int64_t)entry_of_token[t] * table_width + pos / page_size];
-  const int G = pack_groups(hd), NB = pack_slices(hd), slot = pos % page_size, token = slot % kPackTokens;
-  const int quad = token / 4, i = token % 4;
-  Eight<T> out;
+__global__ __launch_bounds__(256) void pack_values_kernel(PackValuesArgs a) {
+  const unsigned piece = blockIdx.x * 256 + threadIdx.x, row = divided(piece, a.per, a.per_inv);
+  const int sub = (int)(piece - row * a.per);
+  const int t = (int)divided(row, 2 * a.nkv, a.heads_inv), h = (int)(row - (unsigned)t * 2 * a.nkv);
+  if (t >= a.num_tokens) return;
+  const bool key = h < a.nkv;
+  const int head = key ? h : h - a.nkv, pos = a.positions[t], entry = a.entry_of_token[t];
+  int count = 1;
+  if (!key) {
+    const int i0 = pos & 3;
+    if (i0 != 0 && t > 0 && a.entry_of_token[t - 1] == entry && a.positions[t - 1] == pos - 1) return;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) out.set(e, 0.f);
-  if (page >= 0) {
-    const unsigned char* block =
-        (key ? k_pages : v_pages) + pack_block(page, nkv, head, page_size, slot, pack_block_bytes(hd));
-    const unsigned* words = (const unsigned*)block;
-    const unsigned char* scale = block + pack_codes_bytes(hd) + (quad * G + sub / 8) * 16;
-    const float step = (float)((const _Float16*)scale)[i];
-    const float zero = -16.f - (float)((const _Float16*)scale)[4 + i];
-    unsigned code[8];
-    if (key) {
-      const unsigned word = pack_unturned<kPackTurnK>(words[(sub % 4 * 16 + token) * NB + sub / 4]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) code[j] = word >> (4 * (j / 2 + 4 * (j % 2))) & 15;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        code[e] = pack_unturned<kPackTurnV>(words[(quad * 16 + sub % 2 * 8 + e) * NB + sub / 4]) >>
-                  (4 * (2 * (sub / 2 % 2) + i / 2 + 4 * (i % 2))) & 15;
+    for (int j = 1; j < 4; ++j) {
+      const int n = min(t + j, a.num_tokens - 1);
+      if (count == j && i0 + j < 4 && t + j < a.num_tokens && a.entry_of_token[n] == entry && a.positions[n] == pos + j)
+        count = j + 1;
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out.set(e, step * ((float)code[e] - zero));
   }
-  out.store((key ? k : v) + ((int64_t)t * nkv + head) * hd + sub * 8);
+  const int page = a.table[(int64_t)entry * a.table_width + (pos >> __builtin_ctz(a.page_size))];
+  const int G = pack_groups(a.hd), NB = pack_slices(a.hd), slot = pos & (a.page_size - 1), token = slot % kPackTokens;
+  const int quad = token / 4, i0 = token % 4;
+  const unsigned char* block = (key ? a.k_pages : a.v_pages) +
+                               pack_block(max(page, 0), a.nkv, head, a.page_size, slot, pack_block_bytes(a.hd));
+  const unsigned* words = (const unsigned*)block;
+  typedef _Float16 eight_h __attribute__((ext_vector_type(8)));
+  const eight_h scale = *(const eight_h*)(block + pack_codes_bytes(a.hd) + (quad * G + sub / 8) * 16);
+  T* dst = (T*)(key ? a.k : a.v) + ((int64_t)t * a.nkv + head) * a.hd + sub * 8;
+  unsigned word[8];
+  if (key) {
+    word[0] = pack_unturned<kPackTurnK>(words[(sub % 4 * 16 + token) * NB + sub / 4]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) word[e] = pack_unturned<kPackTurnV>(words[(quad * 16 + sub % 2 * 8 + e) * NB + sub / 4]);
+  }
+  for (int j = 0; j < count; ++j) {
+    const int i = i0 + j;
+    const float step = page >= 0 ? (float)(i == 0 ? scale[0] : i == 1 ? scale[1] : i == 2 ? scale[2] : scale[3]) : 0.f;
+    const float bias = (float)(i == 0 ? scale[4] : i == 1 ? scale[5] : i == 2 ? scale[6] : scale[7]);
+    const int at = 4 * (2 * (sub / 2 % 2) + i / 2 + 4 * (i % 2));
+    Eight<T> out;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned code = key ? word[0] >> (4 * (e / 2 + 4 * (e % 2))) & 15 : word[e] >> at & 15;
+      out.set(e, page >= 0 ? step * ((float)code + 16.f + bias) : 0.f);
+    }
+    out.store(dst + (int64_t)j * a.nkv * a.hd);
+  }
 }
 
 extern "C" int ts_pack_values(const void* k_pages, const void* v_pages, void* k, void* v, int type, const int* positions,
@@ -270,12 +285,15 @@ extern "C" int ts_pack_values(const void* k_pages, const void* v_pages, void* k,
   if (num_tokens <= 0) return 0;
   if (!pack_fits(hd, page_size)) TS_FAIL("pack_values: head_dim=%d, page_size=%d not built", hd, page_size);
   if (nkv <= 0 || !table || table_width <= 0) TS_FAIL("pack_values: nkv=%d, block table of width %d", nkv, table_width);
+  if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15)
+    TS_FAIL("pack_values: tensors must be 16-byte aligned");
   const int64_t pieces = (int64_t)num_tokens * 2 * nkv * (hd / 8), blocks = (pieces + 255) / 256;
-  if (blocks > 2147483647LL) TS_FAIL("pack_values: too many tokens");
+  if (pieces > 2147483647LL - 256) TS_FAIL("pack_values: too many tokens");
+  const unsigned per = hd / 8, heads = 2 * nkv;
+  const PackValuesArgs a{(const unsigned char*)k_pages, (const unsigned char*)v_pages, k, v, positions, entry_of_token,
+                         table, table_width, num_tokens, nkv, hd, page_size, per, inverse32(per), inverse32(heads)};
   TS_DISPATCH_TYPE(type, T,
-      hipLaunchKernelGGL(pack_values_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream,
-                         (const unsigned char*)k_pages, (const unsigned char*)v_pages, (T*)k, (T*)v, positions,
-                         entry_of_token, table, table_width, pieces, nkv, hd, page_size));
+      hipLaunchKernelGGL(pack_values_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream, a));
   TS_CHECK_LAUNCH("pack_values");
   return 0;
 }
