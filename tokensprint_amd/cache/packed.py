@@ -10,6 +10,8 @@ What a cache holds is read back with the provider's `kv_values`.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 TOKENS = 16             # tokens of a block
@@ -32,6 +34,7 @@ def check_packed(head_dim: int, page_size: int) -> None:
                          f"from {TOKENS}")
 
 
+@lru_cache(maxsize=1024)
 def packed_pages_shape(num_pages: int, num_kv_heads: int, page_size: int,
                        head_dim: int) -> tuple[int, int, int, int]:
     """Shape of the uint8 tensor that holds keys, and of the one that holds values."""

@@ -109,3 +109,22 @@ extern "C" int ts_gemm_int8(const void* x, const float* a_scale, const void* w, 
   if (pair) return c_type == TS_BF16 ? launch_int8<bf16_t, true>(a, stream) : launch_int8<float, true>(a, stream);
   return c_type == TS_BF16 ? launch_int8<bf16_t, false>(a, stream) : launch_int8<float, false>(a, stream);
 }
+
+extern "C" int ts_quantize_rows(const void* x, int type, void* codes, float* scales, int M, int K, int row,
+                                hipStream_t stream);
+extern "C" int ts_norm_quantize_rows(const float* resid, const void* delta, int delta_type, const float* norm_w, float eps,
+                                     float* resid_out, void* codes, float* scales, int M, int K, int row,
+                                     hipStream_t stream);
+
+// Rows into 8 bits and their product.  `norm_w` null: x as it is; else x is the float32 stream, `delta` (or null) is
+// added to it, the sum goes into `resid_out` and the rows are normed.  `rows`: M (row + 4) bytes of scratch memory.
+extern "C" int ts_linear_int8(const void* x, int x_type, const void* delta, int delta_type, const float* norm_w, float eps,
+                              float* resid_out, void* rows, const void* w, const float* w_scale, void* c, int c_type,
+                              int M, int N, int K, int row, int pair, float limit, hipStream_t stream) {
+  if (M <= 0) return 0;
+  float* scales = (float*)((char*)rows + (int64_t)M * row);
+  const int rc = norm_w ? ts_norm_quantize_rows((const float*)x, delta, delta_type, norm_w, eps, resid_out, rows, scales, M,
+                                                K, row, stream)
+                        : ts_quantize_rows(x, x_type, rows, scales, M, K, row, stream);
+  return rc ? rc : ts_gemm_int8(rows, scales, w, w_scale, c, c_type, M, N, row, pair, limit, 0, stream);
+}

@@ -96,6 +96,18 @@ class PromptAttentionArgs(Structure):
     ]
 
 
+#: arguments of entry points that a step calls often: addresses, whole numbers, float32s
+_LETTERS = {"p": c_void_p, "i": c_int, "f": c_float}
+_ARGUMENTS = {
+    "ts_pack_store": "ppippppp" + "iiiii" + "p",
+    "ts_pack_values": "ppppi" + "ppp" + "iiiii" + "p",
+    "ts_quantize_rows": "pi" + "pp" + "iii" + "p",
+    "ts_norm_quantize_rows": "ppipf" + "ppp" + "iii" + "p",
+    "ts_gemm_int8": "ppppp" + "iiiii" + "f" + "i" + "p",
+    "ts_linear_int8": "pi" + "pipfp" + "pppp" + "iiiii" + "if" + "p",
+}
+
+
 def _load_library() -> ctypes.CDLL:
     path = find_library()
     if path is None:
@@ -104,6 +116,9 @@ def _load_library() -> ctypes.CDLL:
     lib.ts_last_error.restype = ctypes.c_char_p
     lib.ts_chunked_scratch.restype = c_int64
     lib.ts_capture_id.restype = c_int64
+    # (with their types named, addresses go in as the numbers that they are, not each in an object of its own)
+    for name, args in _ARGUMENTS.items():
+        getattr(lib, name).argtypes = [_LETTERS[c] for c in args]
     if lib.ts_abi_version() != ABI_VERSION:
         raise KernelError(f"{path} has interface version {lib.ts_abi_version()}, "
                           f"this package needs {ABI_VERSION}")
@@ -204,6 +219,9 @@ class HipOps:
         key = stream, self.lib.ts_capture_id(c_void_p(stream)) if stream else 0
         counts = self._count_arrays.get(key)
         if counts is None or counts.numel() < n:
+            if key[1]:               # what earlier captures used belongs to their graphs alone
+                for other in [k for k in self._count_arrays if k[1] not in (0, key[1])]:
+                    del self._count_arrays[other]
             counts = torch.zeros(max(n, 4096), dtype=torch.int32, device=self.device)
             self._count_arrays[key] = counts
         return counts
@@ -838,9 +856,8 @@ class HipOps:
         rows go into the product in 8 bits, and the returned stream is another tensor unless
         there is nothing to add."""
         if weight.__class__ is Int8Weight:
-            rows, resid = self.norm_quantize_rows(resid, delta, norm_weight, eps)
-            product = self.linear_silu_mul if silu_mul else self.linear
-            return product(rows, weight, out_dtype), resid
+            delta, out = self._normed(resid, delta, norm_weight)
+            return self._int8_linear(resid, delta, norm_weight, eps, out, weight, out_dtype, silu_mul, None), out
         self._check("resid", resid, torch.float32, ndim=2)
         if isinstance(delta, PreparedRows):     # already added in, by linear_into_stream
             return self._prepared_linear(resid, delta, norm_weight, eps, weight, out_dtype,
@@ -918,8 +935,8 @@ class HipOps:
         row = self._int8_row(K)
         codes = torch.empty(M, row, dtype=torch.int8, device=self.device)
         scales = torch.empty(M, dtype=torch.float32, device=self.device)
-        self._call(self.lib.ts_quantize_rows, _ptr(x), _TYPE_CODE[x.dtype], _ptr(codes), _ptr(scales),
-                   M, K, row, self._stream())
+        self._call(self.lib.ts_quantize_rows, x.data_ptr(), _TYPE_CODE[x.dtype], codes.data_ptr(),
+                   scales.data_ptr(), M, K, row, self._raw_stream(self._device_index))
         return kind(codes, scales, K)
 
     @staticmethod
@@ -928,43 +945,75 @@ class HipOps:
             raise ValueError(f"rows in 8 bits: {K} elements, 1 to 131,072 are served")
         return row_bytes(K)
 
+    def _normed(self, resid, delta, norm_weight):
+        """(delta, or None; the stream's tensor after the add) of a norm whose rows go into 8 bits."""
+        self._check("resid", resid, torch.float32, ndim=2)
+        self._check("norm weight", norm_weight, torch.float32, shape=(resid.shape[1],))
+        if delta is None:
+            return None, resid
+        delta = self._rows(delta)
+        self._check("delta", delta, self._FLOATS, shape=resid.shape)
+        return delta, torch.empty_like(resid)
+
     def norm_quantize_rows(self, resid, delta, norm_weight, eps):
         """(RMSNorm(resid + delta) as Int8Rows, resid + delta): `delta` may be None, and the returned
         stream is then `resid` itself, else a new tensor.  The normed rows are quantised in
         float32, not rounded to another type first."""
-        self._check("resid", resid, torch.float32, ndim=2)
+        delta, out = self._normed(resid, delta, norm_weight)
         M, K = resid.shape
-        self._check("norm weight", norm_weight, torch.float32, shape=(K,))
-        out, row = resid, self._int8_row(K)
-        if delta is not None:
-            delta = self._rows(delta)
-            self._check("delta", delta, self._FLOATS, shape=resid.shape)
-            out = torch.empty_like(resid)
+        row = self._int8_row(K)
         codes = torch.empty(M, row, dtype=torch.int8, device=self.device)
         scales = torch.empty(M, dtype=torch.float32, device=self.device)
-        self._call(self.lib.ts_norm_quantize_rows, _ptr(resid), _ptr(delta),
-                   _TYPE_CODE[delta.dtype] if delta is not None else 0, _ptr(norm_weight),
-                   c_float(eps), _ptr(out if delta is not None else None), _ptr(codes), _ptr(scales),
-                   M, K, row, self._stream())
+        self._call(self.lib.ts_norm_quantize_rows, resid.data_ptr(),
+                   None if delta is None else delta.data_ptr(), 0 if delta is None else _TYPE_CODE[delta.dtype],
+                   norm_weight.data_ptr(), eps, None if delta is None else out.data_ptr(), codes.data_ptr(),
+                   scales.data_ptr(), M, K, row, self._raw_stream(self._device_index))
         return Int8Rows(codes, scales, K), out
+
+    def _int8_weight(self, weight, K, out_dtype, pair):
+        """(columns of the product, bytes of a row) of a weight that rows of K elements may meet."""
+        if out_dtype not in _TYPE_CODE:
+            raise TypeError(f"a product in 8 bits cannot give {out_dtype}")
+        rows = weight.codes.shape[0]
+        if weight.width != K or (pair and rows % 2):
+            raise ValueError(f"a product in 8 bits: rows of {K}, weight {tuple(weight.shape)}")
+        row = self._int8_row(K)
+        self._check("weight codes", weight.codes, torch.int8, shape=(rows, row))
+        self._check("weight scales", weight.scales, torch.float32, shape=(rows,))
+        return rows // 2 if pair else rows, row
 
     def _int8_product(self, x, weight, out_dtype, pair=False, unit=None, tile=0):
         """`tile` as in `gemm_tiled`; 9: the kernel for few rows."""
         if not isinstance(x, Int8Rows):
+            if tile == 0:
+                x = self._rows(x)
+                self._check("x", x, self._FLOATS, ndim=2)
+                return self._int8_linear(x, None, None, 0.0, None, weight, out_dtype, pair, unit)
             x = self.quantize_rows(x)
-        if out_dtype not in _TYPE_CODE:
-            raise TypeError(f"a product in 8 bits cannot give {out_dtype}")
-        if x.width != weight.width or (pair and weight.codes.shape[0] % 2):
-            raise ValueError(f"a product in 8 bits: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
-        for name, t in (("x", x), ("weight", weight)):
-            rows = t.codes.shape[0]
-            self._check(name + " codes", t.codes, torch.int8, shape=(rows, self._int8_row(t.width)))
-            self._check(name + " scales", t.scales, torch.float32, shape=(rows,))
-        M, N = x.codes.shape[0], weight.codes.shape[0] // 2 if pair else weight.codes.shape[0]
+        N, row = self._int8_weight(weight, x.width, out_dtype, pair)
+        M = x.codes.shape[0]
+        self._check("x codes", x.codes, torch.int8, shape=(M, row))
+        self._check("x scales", x.scales, torch.float32, shape=(M,))
         out = torch.empty(M, N, dtype=out_dtype, device=self.device)
-        self._call(self.lib.ts_gemm_int8, _ptr(x.codes), _ptr(x.scales), _ptr(weight.codes),
-                   _ptr(weight.scales), _ptr(out), _TYPE_CODE[out_dtype], M, N, x.codes.shape[1],
-                   int(pair), unit or c_float(0.0), tile, self._stream())
+        self._call(self.lib.ts_gemm_int8, x.codes.data_ptr(), x.scales.data_ptr(), weight.codes.data_ptr(),
+                   weight.scales.data_ptr(), out.data_ptr(), _TYPE_CODE[out_dtype], M, N, row, int(pair),
+                   unit or 0.0, tile, self._raw_stream(self._device_index))
+        return out
+
+    def _int8_linear(self, x, delta, norm_weight, eps, stream_out, weight, out_dtype, pair, unit):
+        """Rows (with a norm weight: of the stream, added to and normed) into 8 bits and their product, in
+        one call."""
+        M, K = x.shape
+        N, row = self._int8_weight(weight, K, out_dtype, pair)
+        out = torch.empty(M, N, dtype=out_dtype, device=self.device)
+        rows = torch.empty(M * (row + 4), dtype=torch.int8, device=self.device)      # numbers, then scales
+        added = delta is not None
+        self._call(self.lib.ts_linear_int8, x.data_ptr(), _TYPE_CODE[x.dtype],
+                   delta.data_ptr() if added else None, _TYPE_CODE[delta.dtype] if added else 0,
+                   None if norm_weight is None else norm_weight.data_ptr(), eps,
+                   stream_out.data_ptr() if added else None, rows.data_ptr(), weight.codes.data_ptr(),
+                   weight.scales.data_ptr(), out.data_ptr(), _TYPE_CODE[out_dtype], M, N, K, row,
+                   int(pair), unit or 0.0, self._raw_stream(self._device_index))
         return out
 
     # ------------------------------------------------------------ q/k preparation
@@ -1090,10 +1139,10 @@ class HipOps:
         self._check("positions", batch.positions, torch.int32, shape=(T,))
         if cache.k_pages.dtype is torch.uint8:
             self._check("entry_of_token", batch.entry_of_token, torch.int32, shape=(T,))
-            self._call(self.lib.ts_pack_store, _ptr(k), _ptr(v), _TYPE_CODE[k.dtype],
-                       _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(batch.positions),
-                       _ptr(batch.entry_of_token), _ptr(table), table.shape[1], T, nkv, hd,
-                       cache.page_size, self._stream())
+            self._call(self.lib.ts_pack_store, k.data_ptr(), v.data_ptr(), _TYPE_CODE[k.dtype],
+                       cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), batch.positions.data_ptr(),
+                       batch.entry_of_token.data_ptr(), table.data_ptr(), table.shape[1], T, nkv, hd,
+                       cache.page_size, self._raw_stream(self._device_index))
             return
         self._call(self.lib.ts_kv_store, _ptr(k), _ptr(v), _TYPE_CODE[k.dtype],
                    _ptr(cache.k_pages), _ptr(cache.v_pages), _TYPE_CODE[cache.k_pages.dtype],
@@ -1113,10 +1162,10 @@ class HipOps:
         self._check("entry_of_token", batch.entry_of_token, torch.int32, shape=(T,))
         k = torch.empty(T, num_kv_heads, head_dim, dtype=out_dtype, device=self.device)
         v = torch.empty_like(k)
-        self._call(self.lib.ts_pack_values, _ptr(cache.k_pages), _ptr(cache.v_pages), _ptr(k),
-                   _ptr(v), _TYPE_CODE[out_dtype], _ptr(batch.positions),
-                   _ptr(batch.entry_of_token), _ptr(table), table.shape[1], T, num_kv_heads,
-                   head_dim, cache.page_size, self._stream())
+        self._call(self.lib.ts_pack_values, cache.k_pages.data_ptr(), cache.v_pages.data_ptr(),
+                   k.data_ptr(), v.data_ptr(), _TYPE_CODE[out_dtype], batch.positions.data_ptr(),
+                   batch.entry_of_token.data_ptr(), table.data_ptr(), table.shape[1], T, num_kv_heads,
+                   head_dim, cache.page_size, self._raw_stream(self._device_index))
         return k, v
 
     # ------------------------------------------------------------ attention
@@ -1137,14 +1186,19 @@ class HipOps:
         if T != batch.num_tokens:
             raise ValueError("q rows differ from the batch's tokens")
         out = torch.empty_like(q)
+        if cache.k_pages.dtype is torch.uint8:
+            m = PackedArgs()
+            self._fill_attention_args(m.base, q, out, batch, table, cache, num_heads, num_kv_heads,
+                                      head_dim, scale, window, sink, chunk, softcap, slopes, q_temp,
+                                      keep_first)
+            self._attention_packed(m, batch, num_heads // num_kv_heads, q.dtype)
+            return out
         a = AttentionArgs()
         self._fill_attention_args(a, q, out, batch, table, cache, num_heads, num_kv_heads,
                                   head_dim, scale, window, sink, chunk, softcap, slopes, q_temp,
                                   keep_first)
         extras = softcap is not None or slopes is not None or q_temp is not None
-        if cache.k_pages.dtype is torch.uint8:
-            self._attention_packed(a, batch, num_heads // num_kv_heads, q.dtype)
-        elif (q.dtype == torch.bfloat16 and cache.k_pages.dtype == torch.bfloat16
+        if (q.dtype == torch.bfloat16 and cache.k_pages.dtype == torch.bfloat16
                 and head_dim % 16 == 0 and head_dim <= 256 and cache.page_size % 4 == 0):
             # (scores with extras: of the kernels for long portions those for pages of a power
             # of two know them)
@@ -1176,27 +1230,33 @@ class HipOps:
                        _TYPE_CODE[cache.k_pages.dtype], self._stream())
         return out
 
-    def _attention_packed(self, a, batch, group, dtype):
+    def _attention_packed(self, m, batch, group, dtype):
         """Attention over a cache of 4 bits: portions of prompts by the kernel that makes tiles in LDS
         (bfloat16, heads of 64 and 128), everything else in tiles of 16 rows (query heads of a key/value
         head x tokens), whose keys are shared out over workgroups where the tiles are few."""
+        a = m.base
         if not a.scale > 0:
             raise ValueError(f"attention over keys of 4 bits: scale={a.scale} must be positive")
-        d, tokens = self.dispatch, 16 // min(group, 16)
-        tall = dtype is torch.bfloat16 and self.lib.ts_packed_prompt_fits(a.hd) == 1
+        d = self.dispatch
+        m.rows_per_token, m.head_blocks = min(group, 16), -(-group // 16)
+        tokens, heads, stream = 16 // m.rows_per_token, a.nkv * m.head_blocks, self._raw_stream(self._device_index)
+        key = "packed", a.hd, dtype
+        found = self._routes.get(key) if self._routes_of is d else None
+        if found is None:
+            found = self._kept_routes()[key] = (
+                dtype is torch.bfloat16 and self.lib.ts_packed_prompt_fits(a.hd) == 1,
+                d.packed_workgroups or self.lib.ts_packed_resident(a.hd, _TYPE_CODE[dtype]))
+        tall, resident = found
         for portions in (True, False):
             count, tiles = self._packed_tiles(batch, portions, 8 * tokens if portions and tall else tokens,
                                               d.packed_portion)
             if count == 0:
                 continue
-            m = PackedArgs()
-            m.base = a
-            m.rows_per_token, m.head_blocks = min(group, 16), -(-group // 16)
             m.num_tiles, m.tiles = count, tiles
-            items = count * a.nkv * m.head_blocks
+            items = count * heads
             if portions and tall:
                 # two sets of wavefronts share an item's keys where items leave units empty
-                self._call(self.lib.ts_packed_prompt, byref(m), 2 if items <= self._units else 1, self._stream())
+                self._call(self.lib.ts_packed_prompt, byref(m), 2 if items <= self._units else 1, c_void_p(stream))
                 continue
             shared = items <= d.packed_items
             if shared:
@@ -1205,14 +1265,13 @@ class HipOps:
                 chunks = -(-keys // 128)
                 if chunks > d.packed_whole:
                     # a workgroup for every 128 keys that there can be, as many as the card holds at a time
-                    m.workgroups = min(items * chunks, d.packed_workgroups
-                                       or self.lib.ts_packed_resident(a.hd, _TYPE_CODE[dtype]))
+                    workgroups = m.workgroups = min(items * chunks, resident)
                     hd = -(-a.hd // 32) * 32
-                    partial = torch.empty(m.workgroups * 32 * (hd + 2), dtype=torch.float32, device=self.device)
-                    m.partial_o = partial.data_ptr()
-                    m.partial_ml = m.partial_o + m.workgroups * 32 * hd * 4
+                    partial = torch.empty(workgroups * 32 * (hd + 2), dtype=torch.float32, device=self.device)
+                    m.partial_o = at = partial.data_ptr()
+                    m.partial_ml = at + workgroups * 32 * hd * 4
                     m.arrivals = self._counts(items).data_ptr()
-            self._call(self.lib.ts_packed_attention, byref(m), _TYPE_CODE[dtype], int(shared), self._stream())
+            self._call(self.lib.ts_packed_attention, byref(m), _TYPE_CODE[dtype], int(shared), c_void_p(stream))
 
     def _packed_tiles(self, batch, portions, tokens, least):
         """(number, device address or None) of the runs of at most `tokens` consecutive tokens of the
