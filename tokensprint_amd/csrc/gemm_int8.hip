@@ -1,94 +1,69 @@
 // Products in 8 bits for few rows, where streaming the weight once is the whole cost, and the entry point of all.
 //
-// A workgroup owns 16 rows of W (16 of each half with PAIR) and up to 64 rows of A; its waves share K out. Both operands go
-// from memory into the layout of v_mfma_i32_16x16x64_i8: a lane takes 64 contiguous bytes of its row
-// an iteration, so four lanes cover 256 and a wave 4 KB of W; the k that a register slot stands for is permuted the
-// same way in both, which a sum of whole numbers does not notice.
+// A workgroup owns 16 rows of W (16 of each half with PAIR) and 16 rows of A; its eight waves share K out.  Both operands
+// go from memory into the layout of v_mfma_i32_16x16x64_i8: of a row, four lanes take 64 contiguous bytes a load, and
+// four loads 256.  (A lane taking 64 contiguous bytes over four loads, which the products' order of k would allow,
+// touched four times as many pieces of memory a load: 16 rows of [2 x 12288, 4096] took 29 us against 20.)
+// W of 16.8 MB that no cache holds takes 6 us for 1 row, 8 for 16 (2.8 and 2.1 TB/s); 50 MB as [4096, 12288] 13 and 18;
+// 100 MB as [2 x 12288, 4096] 24 and 28 (4.2 and 3.6 TB/s).  Four waves lose 10 % in the first two.
 #include "gemm_int8.h"
 
-// MT: 16-row tiles of A; NW: waves along K.
-template <int MT, int NW, typename TC, bool PAIR>
-__global__ __launch_bounds__(NW * kWave) void gemm_int8_kernel(Int8Args a) {
-  constexpr int HALVES = PAIR ? 2 : 1;
-  __shared__ i32x4 red[NW - 1][HALVES][MT][kWave];
+constexpr int kWavesAlongK = 8;
+
+template <typename TC, bool PAIR>
+__global__ __launch_bounds__(kWavesAlongK* kWave) void gemm_int8_kernel(Int8Args a) {
+  constexpr int HALVES = PAIR ? 2 : 1, NW = kWavesAlongK;
+  __shared__ i32x4 red[NW - 1][HALVES][kWave];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int r = lane % 16, g = lane / 16;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (MT * 16);
-  const signed char* w = a.w + (int64_t)min(n0 + r, a.N - 1) * a.row + g * 64;
-  const signed char* x[MT];
+  const int n0 = blockIdx.x * 16, m = blockIdx.y * 16 + r;
+  const signed char* w = a.w + (int64_t)min(n0 + r, a.N - 1) * a.row + g * 16;
+  const signed char* x = a.a + (int64_t)min(m, a.M - 1) * a.row + g * 16;
+  i32x4 acc[HALVES];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) x[t] = a.a + (int64_t)min(m0 + t * 16 + r, a.M - 1) * a.row + g * 64;
-  i32x4 acc[HALVES][MT];
-#pragma unroll
-  for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[h][t] = i32x4{0, 0, 0, 0};
-#pragma unroll 2
+  for (int h = 0; h < HALVES; ++h) acc[h] = i32x4{0, 0, 0, 0};
   for (int k = wave * 256; k < a.row; k += NW * 256) {
-    i32x4 wv[HALVES][4];
+    i32x4 wv[HALVES][4], xv[4];
 #pragma unroll
     for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) wv[h][s] = *(const i32x4*)(w + (int64_t)h * a.N * a.row + k + s * 16);
+      for (int s = 0; s < 4; ++s) wv[h][s] = *(const i32x4*)(w + (int64_t)h * a.N * a.row + k + s * 64);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      i32x4 xv[4];
+    for (int s = 0; s < 4; ++s) xv[s] = *(const i32x4*)(x + k + s * 64);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) xv[s] = *(const i32x4*)(x[t] + k + s * 16);
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h)
-          acc[h][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[h][s], xv[s], acc[h][t], 0, 0, 0);
-    }
+      for (int h = 0; h < HALVES; ++h) acc[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[h][s], xv[s], acc[h], 0, 0, 0);
   }
   if (wave > 0) {
 #pragma unroll
-    for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-      for (int t = 0; t < MT; ++t) red[wave - 1][h][t][lane] = acc[h][t];
+    for (int h = 0; h < HALVES; ++h) red[wave - 1][h][lane] = acc[h];
   }
   __syncthreads();
   if (wave > 0) return;
 #pragma unroll
   for (int o = 0; o < NW - 1; ++o)
 #pragma unroll
-    for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-      for (int t = 0; t < MT; ++t) acc[h][t] += red[o][h][t][lane];
-  // lane holds the sums of columns n0 + 4 g + i of row m0 + 16 t + r
+    for (int h = 0; h < HALVES; ++h) acc[h] += red[o][h][lane];
+  // lane holds the sums of columns n0 + 4 g + i of row m
   const int n = n0 + g * 4;
-  if (n >= a.N) return;
-  float scale[HALVES][4];
+  if (n >= a.N || m >= a.M) return;
+  const float row = a.a_scale[m];
+  f32x4 v;
 #pragma unroll
-  for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) scale[h][i] = a.w_scale[h * a.N + min(n + i, a.N - 1)];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int m = m0 + t * 16 + r;
-    if (m >= a.M) continue;
-    const float row = a.a_scale[m];
-    f32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = (float)acc[0][t][i] * scale[0][i] * row;
-      if constexpr (PAIR) v[i] = gated_unit(v[i], (float)acc[1][t][i] * scale[1][i] * row, a.limit);
-    }
-    store4<TC>((TC*)a.c + (int64_t)m * a.N + n, v, a.N - n);
+  for (int i = 0; i < 4; ++i) {
+    const int column = min(n + i, a.N - 1);
+    v[i] = (float)acc[0][i] * a.w_scale[column] * row;
+    if constexpr (PAIR) v[i] = gated_unit(v[i], (float)acc[1][i] * a.w_scale[a.N + column] * row, a.limit);
   }
+  store4<TC>((TC*)a.c + (int64_t)m * a.N + n, v, a.N - n);
 }
 
 template <typename TC, bool PAIR>
 static int launch_int8(const Int8Args& a, hipStream_t stream) {
-  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-  const dim3 grid((a.N + 15) / 16, (a.M + mt * 16 - 1) / (mt * 16));
+  const dim3 grid((a.N + 15) / 16, (a.M + 15) / 16);
   if (grid.y > 65535) TS_FAIL("gemm_int8: M=%d rows of %d bytes", a.M, a.row);
-#define TS_INT8(MT) hipLaunchKernelGGL((gemm_int8_kernel<MT, 4, TC, PAIR>), grid, dim3(4 * kWave), 0, stream, a)
-  if (mt == 1) TS_INT8(1);
-  else if (mt == 2) TS_INT8(2);
-  else TS_INT8(4);
-#undef TS_INT8
+  hipLaunchKernelGGL((gemm_int8_kernel<TC, PAIR>), grid, dim3(kWavesAlongK * kWave), 0, stream, a);
   TS_CHECK_LAUNCH("gemm_int8");
   return 0;
 }
@@ -105,7 +80,13 @@ extern "C" int ts_gemm_int8(const void* x, const float* a_scale, const void* w, 
   const Int8Args a{(const signed char*)x, (const signed char*)w, a_scale, w_scale, c, M, N, row, limit};
   const bool many = gemm_int8_tiled_fits(M, N, row, pair != 0);
   if (tile > 0 && tile < 9 && !many) TS_FAIL("gemm_int8: M=%d N=%d rows of %d bytes not taken in tiles", M, N, row);
-  if (tile == 0 ? M > 64 && many : tile < 9) return gemm_int8_tiled(a, c_type, pair != 0, tile, stream);
+  // Tiles from 5 rows on where the kernel above would be more than two workgroups a unit, of which every one reads its
+  // rows of A for 16 rows of W alone (W [24576, 4096]: 1 row 24 us here, 26 in tiles; 16 rows 30 and 27.  [12288, 4096]:
+  // 8 rows 15 and 15, 16 rows 17 and 15.  [4096, 4096]: 16 rows 8 and 10, 32 rows 10.5 and 10.5, 64 rows 18 and 11.
+  // [1024, 4096]: 64 rows 6.0 and 7.5, 256 rows 16 and 7.4).
+  const int64_t workgroups = ((pair ? 2ll * N : N) + 15) / 16 * ((M + 15) / 16);
+  const bool few = M <= 4 || workgroups <= 512;
+  if (tile == 0 ? many && !few : tile < 9) return gemm_int8_tiled(a, c_type, pair != 0, tile, stream);
   if (pair) return c_type == TS_BF16 ? launch_int8<bf16_t, true>(a, stream) : launch_int8<float, true>(a, stream);
   return c_type == TS_BF16 ? launch_int8<bf16_t, false>(a, stream) : launch_int8<float, false>(a, stream);
 }
