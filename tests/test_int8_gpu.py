@@ -227,3 +227,19 @@ def test_refusals(ops, gpu_device):
         ops.quantize_weight(x.cpu())
     with pytest.raises(ValueError):
         ops.norm_quantize_rows(x.float(), x[:2], torch.ones(64, device=gpu_device), 1e-6)
+
+
+@pytest.mark.parametrize("k", [64, 4096, 5000])
+@pytest.mark.parametrize("rows", [1, 1000])
+@pytest.mark.parametrize("top", [1e-35, 3e-37, 2e-38])
+def test_rows_of_tiny_elements(ops, rows, k, top):
+    """Scales below what a reciprocal in float32 has room for: still the nearest whole numbers."""
+    x = (torch.rand(rows, k, dtype=torch.float64) * 2 - 1) * top
+    x[:, 0] = top
+    x = x.float()
+    got = ops.quantize_rows(x.cuda())
+    scale = got.scales.cpu().double()
+    # (a scale below 2^-126 has fewer bits: half a step of 2^-149)
+    assert ((scale - x.double().abs().amax(1) / 127).abs() <= scale * 2.0**-24 + 2.0**-150).all()
+    ratio = x.double() / scale[:, None]
+    assert ((got.codes.cpu()[:, :k].double() - ratio.clamp(-127, 127)).abs() <= 0.5).all()

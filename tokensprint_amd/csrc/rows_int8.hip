@@ -4,8 +4,8 @@
 // type or written in it.  A row with an infinity or a NaN has a scale that is neither finite, so its products
 // are not numbers either.
 //
-// A workgroup takes a row, eight neighbouring elements a piece: bound by memory for many rows, by one trip and
-// two meetings of the workgroup for few.  Codes go into rows of `row` bytes (a multiple of 256, zeros behind the
+// A workgroup takes a row, eight neighbouring elements a piece: bound by memory for many rows (8,192 of 5,120 28 us, 4.5
+// TB/s; with the add and the norm 87 us, 5.3 TB/s), by one trip and two meetings of the workgroup for few (3.3 us).  Codes go into rows of `row` bytes (a multiple of 256, zeros behind the
 // last element), which is what the products walk in.
 #include "common.h"
 
@@ -23,11 +23,11 @@ struct QuantRowsArgs {
 // The larger, or NaN if either is.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-template <int N>
 __device__ __forceinline__ float block_largest(float v, float* scratch) {
 #pragma unroll
   for (int o = kWave / 2; o > 0; o >>= 1) v = larger(v, __shfl_xor(v, o, kWave));
-  const int waves = (blockDim.x + kWave - 1) / kWave;
+  const int waves = blockDim.x / kWave;
+  if (waves == 1) return v;
   if (threadIdx.x % kWave == 0) scratch[threadIdx.x / kWave] = v;
   __syncthreads();
   v = 0.f;
@@ -35,14 +35,52 @@ __device__ __forceinline__ float block_largest(float v, float* scratch) {
   return v;
 }
 
-__device__ __forceinline__ int code8(float x, float scale, float inv) {
-  return (int)fminf(fmaxf(nearest_whole(x, scale, inv), -127.f), 127.f);
+// What turns a row's elements into numbers: about 1 / scale; of a scale so small that this would not be a float32
+// number, scale and elements times 2^64 first.
+struct RowScale {
+  float scale, inv, lift;
+  bool plain;              // the fast way is exact enough (see codes8)
+};
+__device__ __forceinline__ RowScale row_scale(float scale) {
+  RowScale r;
+  r.lift = scale < 0x1p-100f ? 0x1p64f : 1.f;
+  r.scale = scale * r.lift;
+  r.inv = scale > 0.f ? 1.f / r.scale : 0.f;
+  r.plain = scale >= 0x1p-100f && scale < __builtin_inff();
+  return r;
+}
+__device__ __forceinline__ int code8(float x, const RowScale& r) {
+  return (int)fminf(fmaxf(nearest_whole(x * r.lift, r.scale, r.inv), -127.f), 127.f);
+}
+
+// Eight numbers in eight bytes.  The quotient by the product with 1 / scale is within 127 x 2^-23 of the right one (two
+// roundings), and its sum with 1.5 x 2^23 is the nearest whole number in the lowest byte; where one of the wave's
+// quotients is so near to a border between two numbers that this might be the other one (or the scale is not an
+// ordinary number), nearest_whole decides for all: 4 % of the pieces of ordinary rows.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], const RowScale& r) {
+  constexpr float kMagic = 12582912.f;
+  unsigned b[8];
+  float off = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float t = fmaf(v[j], r.inv, kMagic);
+    off = fmaxf(off, fabsf(fmaf(v[j], r.inv, kMagic - t)));
+    b[j] = __float_as_uint(t);
+  }
+  if (__builtin_amdgcn_ballot_w64(off > 0.49996f || !r.plain) != 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = r.scale > 0.f ? (unsigned)code8(v[j], r) : 0u;
+  }
+  auto four = [](unsigned x, unsigned y, unsigned z, unsigned w) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400u), __builtin_amdgcn_perm(y, x, 0x0c0c0400u), 0x05040100u);
+  };
+  return make_uint2(four(b[0], b[1], b[2], b[3]), four(b[4], b[5], b[6], b[7]));
 }
 
 // CH pieces of eight elements a thread, all in registers; CH = 0: rows of any length and alignment, an element at a
 // time, walked once for each of the sums.
 template <typename T, typename TD, bool NORM, int CH>
-__global__ __launch_bounds__(1024) void quant_rows_kernel(QuantRowsArgs a) {
+__global__ __launch_bounds__(CH > 4 ? 512 : 1024) void quant_rows_kernel(QuantRowsArgs a) {
   __shared__ float scratch[16], sums[16];
   const int64_t m = blockIdx.x;
   const T* x = (const T*)a.x + m * a.K;
@@ -52,57 +90,62 @@ __global__ __launch_bounds__(1024) void quant_rows_kernel(QuantRowsArgs a) {
     typedef T eight __attribute__((ext_vector_type(8)));
     typedef TD eight_d __attribute__((ext_vector_type(8)));
     typedef float eight_f __attribute__((ext_vector_type(8)));
-    float v[CH][8];
-    eight raw[CH];
-    eight_d more[CH];
-    eight_f w[CH];
     auto at = [&](int c) { return (c * (int)blockDim.x + (int)threadIdx.x) * 8; };
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int e = min(at(c), a.K - 8);                    // behind the row's end its last piece again, dropped
-      raw[c] = *(const eight*)(x + e);
-      if (NORM && delta) more[c] = *(const eight_d*)(delta + e);
-      if (NORM) w[c] = *(const eight_f*)(a.norm_w + e);
-    }
-    float sq = 0.f, top = 0.f;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const bool there = at(c) < a.K;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[c][j] = there ? to_f32(raw[c][j]) : 0.f;
-        if (NORM && delta) v[c][j] += there ? to_f32(more[c][j]) : 0.f;
-        if (NORM) sq = fmaf(v[c][j], v[c][j], sq);
-      }
-      if (NORM && a.resid_out && there) {
-        eight_f out;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) out[j] = v[c][j];
-        *(eight_f*)(a.resid_out + m * a.K + at(c)) = out;
-      }
-    }
+    eight raw[CH];
+    float v[NORM ? CH : 1][8], top = 0.f;
     if constexpr (NORM) {
+      eight_d more[CH];
+      eight_f w[CH];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int e = min(at(c), a.K - 8);                  // behind the row's end its last piece again, dropped
+        raw[c] = *(const eight*)(x + e);
+        if (delta) more[c] = *(const eight_d*)(delta + e);
+        w[c] = *(const eight_f*)(a.norm_w + e);
+      }
+      float sq = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const bool there = at(c) < a.K;
+        eight_f sum;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[c][j] = there ? to_f32(raw[c][j]) : 0.f;
+          if (delta) v[c][j] += there ? to_f32(more[c][j]) : 0.f;
+          sq = fmaf(v[c][j], v[c][j], sq);
+          sum[j] = v[c][j];
+        }
+        if (a.resid_out && there) *(eight_f*)(a.resid_out + m * a.K + at(c)) = sum;
+      }
       const float rstd = rsqrtf(block_sum(sq, sums) / (float)a.K + a.eps);
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[c][j] *= rstd * w[c][j];
+        for (int j = 0; j < 8; ++j) {
+          v[c][j] *= rstd * w[c][j];
+          top = larger(top, at(c) < a.K ? fabsf(v[c][j]) : 0.f);
+        }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) raw[c] = *(const eight*)(x + min(at(c), a.K - 8));
+#pragma unroll
+      for (int c = 0; c < CH; ++c)                          // (the last piece again changes nothing)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = larger(top, fabsf(to_f32(raw[c][j])));
     }
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = larger(top, at(c) < a.K ? fabsf(v[c][j]) : 0.f);
-    const float scale = block_largest<0>(top, scratch) / 127.f, inv = scale > 0.f ? 1.f / scale : 0.f;
+    const float scale = block_largest(top, scratch) / 127.f;
+    const RowScale by = row_scale(scale);
     if (threadIdx.x == 0) a.scales[m] = scale;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       if (at(c) >= a.row) continue;
-      uint64_t packed = 0;                                  // zeros behind the row's end
-      if (at(c) < a.K && scale > 0.f) {
+      if constexpr (!NORM) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) packed |= (uint64_t)(unsigned char)code8(v[c][j], scale, inv) << (8 * j);
+        for (int j = 0; j < 8; ++j) v[0][j] = to_f32(raw[c][j]);
       }
-      *(uint64_t*)(codes + at(c)) = packed;
+      uint2 packed = codes8(v[NORM ? c : 0], by);
+      if (at(c) >= a.K) packed = make_uint2(0, 0);          // zeros behind the row's end
+      *(uint2*)(codes + at(c)) = packed;
     }
   } else {
     auto value = [&](int e) {
@@ -123,10 +166,11 @@ __global__ __launch_bounds__(1024) void quant_rows_kernel(QuantRowsArgs a) {
     auto normed = [&](int e) { return NORM ? value(e) * (rstd * a.norm_w[e]) : value(e); };
     float top = 0.f;
     for (int e = threadIdx.x; e < a.K; e += blockDim.x) top = larger(top, fabsf(normed(e)));
-    const float scale = block_largest<0>(top, scratch) / 127.f, inv = scale > 0.f ? 1.f / scale : 0.f;
+    const float scale = block_largest(top, scratch) / 127.f;
+    const RowScale by = row_scale(scale);
     if (threadIdx.x == 0) a.scales[m] = scale;
     for (int e = threadIdx.x; e < a.row; e += blockDim.x)
-      codes[e] = e < a.K && scale > 0.f ? (signed char)code8(normed(e), scale, inv) : (signed char)0;
+      codes[e] = e < a.K && scale > 0.f ? (signed char)code8(normed(e), by) : (signed char)0;
   }
 }
 
@@ -136,11 +180,20 @@ static int launch_quant_rows(const QuantRowsArgs& a, hipStream_t stream) {
   const int pieces = a.row / 8;
 #define TS_ROWS(CH, THREADS) \
   hipLaunchKernelGGL((quant_rows_kernel<T, TD, NORM, CH>), dim3((unsigned)a.M), dim3(THREADS), 0, stream, a)
-  // rows of up to 8,192 elements one piece a thread; longer ones more
+  // Few rows, and rows with a norm: a thread a piece, up to 1,024 threads (16 rows of 4,096: 3.3 us, with 256 threads 4.0;
+  // 16,384 with the norm 134 us, 5.5 TB/s, and 137).  Many rows without one: 256 threads and more loads in flight
+  // for each, so that a unit holds more rows between their first load and their last store (8,192 rows
+  // of 5,120: 28 us, 4.5 TB/s; with 640 threads 38; with 64 31).
+  const int most = NORM || a.M <= 512 ? 1024 : pieces <= 1536 ? 256 : 512;
+  const int each = (pieces + most - 1) / most, threads = ((pieces + each - 1) / each + 63) / 64 * 64;
   if (a.K % 8 || (used & 15) || pieces > 4096) TS_ROWS(0, 512);
-  else if (pieces <= 1024) TS_ROWS(1, (pieces + 63) / 64 * 64);
-  else if (pieces <= 2048) TS_ROWS(2, 1024);
-  else TS_ROWS(4, 1024);
+  else if (each == 1) TS_ROWS(1, threads);
+  else if (each == 2) TS_ROWS(2, threads);
+  else if constexpr (NORM) TS_ROWS(4, threads);
+  else if (each == 3) TS_ROWS(3, threads);
+  else if (each == 4) TS_ROWS(4, threads);
+  else if (each <= 6) TS_ROWS(6, threads);
+  else TS_ROWS(8, threads);
 #undef TS_ROWS
   TS_CHECK_LAUNCH("quantize_rows");
   return 0;
