@@ -65,52 +65,77 @@ struct PackGroup {
 };
 
 // The group of the eight lanes that hold 64 elements between them, eight each (`v`; elements that are not there are
-// zeros), and this lane's codes.  A quotient by the estimate of 1 / step is off by less than 2^-18, so a code is the whole
-// number next to it unless that is nearly half a step away; where one of a wavefront's is, all are worked out with what is
-// left over (exactly: ties to even), and where one is no finite number, they are made one.
-__device__ __forceinline__ PackGroup pack_eight(float (&v)[8], unsigned (&code)[8]) {
-  constexpr float kMost = 3.4028234663852886e38f;
-  float none = 0.f;                                            // NaN if an element is not finite
-#pragma unroll
-  for (int j = 0; j < 8; ++j) none = fmaf(v[j], 0.f, none);
-  if (__builtin_expect(__builtin_amdgcn_ballot_w64(none != none) != 0, 0)) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] == v[j] ? fminf(fmaxf(v[j], -kMost), kMost) : 0.f;
-  }
-  float lo = fminf(fminf(v[0], v[1]), 0.f), hi = fmaxf(fmaxf(v[0], v[1]), 0.f);
-#pragma unroll
-  for (int j = 2; j < 8; j += 2) {
-    lo = fminf(fminf(lo, v[j]), v[j + 1]);
-    hi = fmaxf(fmaxf(hi, v[j]), v[j + 1]);
-  }
+// zeros), and this lane's codes, in the order that `place` gives: element j's in bits 4 place(j) on.  A quotient by the
+// estimate of 1 / step is off by less than 2^-18, so a code is the whole number next to it (which adding 1.5 x 2^23 leaves in
+// the lowest bits) unless that is nearly half a step away; where one of a wavefront's is, all are worked out with what
+// is left over (exactly: ties to even), and where one is no finite number, they are made one.
+template <typename PLACE>
+__device__ __forceinline__ PackGroup pack_eight(float (&v)[8], unsigned& word, PLACE place) {
+  constexpr float kMost = 3.4028234663852886e38f, kMagic = 12582912.f;
   // (the neighbour's, the other pair's, then the other four's: lane moves, not trips through LDS)
   auto from = [](float x, auto how) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(how)::value, 0xf, 0xf, true));
   };
-  lo = fminf(lo, from(lo, std::integral_constant<int, 0xB1>{})), hi = fmaxf(hi, from(hi, std::integral_constant<int, 0xB1>{}));
-  lo = fminf(lo, from(lo, std::integral_constant<int, 0x4E>{})), hi = fmaxf(hi, from(hi, std::integral_constant<int, 0x4E>{}));
-  lo = fminf(lo, from(lo, std::integral_constant<int, 0x141>{})), hi = fmaxf(hi, from(hi, std::integral_constant<int, 0x141>{}));
+  float lo, hi;
+  auto range = [&]() {                                         // NaN if an element is
+    lo = hi = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      lo = __builtin_elementwise_minimum(__builtin_elementwise_minimum(lo, v[j]), v[j + 1]);
+      hi = __builtin_elementwise_maximum(__builtin_elementwise_maximum(hi, v[j]), v[j + 1]);
+    }
+    auto both = [&](auto how) {
+      lo = __builtin_elementwise_minimum(lo, from(lo, how)), hi = __builtin_elementwise_maximum(hi, from(hi, how));
+    };
+    both(std::integral_constant<int, 0xB1>{});
+    both(std::integral_constant<int, 0x4E>{});
+    both(std::integral_constant<int, 0x141>{});
+  };
+  range();
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(hi - lo <= kMost)) != 0, 0)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] == v[j] ? fminf(fmaxf(v[j], -kMost), kMost) : 0.f;
+    range();
+  }
   PackGroup p;
   p.step = (_Float16)fminf((hi - lo) / 15.f, 65504.f);
   const float step = (float)p.step, inv = step > 0.f ? __builtin_amdgcn_rcpf(step) : 0.f;
-  float c[8], off;
   p.zero = rintf(-lo * inv);
-  off = fabsf(fmaf(-lo, inv, -p.zero));
+  float off = fabsf(fmaf(-lo, inv, -p.zero)), c[8];
+  p.zero = fminf(p.zero, 15.f);                                // (steps of few bits)
+  const float one = kMagic + p.zero;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float x = v[j] * inv;
-    c[j] = rintf(x);
-    off = fmaxf(off, fabsf(x - c[j]));
+    c[j] = fmaf(v[j], inv, one);
+    off = fmaxf(off, fabsf(fmaf(v[j], inv, one - c[j])));
   }
   if (__builtin_amdgcn_ballot_w64(off > 0.4999f || step >= 65504.f) != 0) {
     p.zero = nearest_whole(-lo, step, inv);
+    p.zero = step > 0.f ? fminf(p.zero, 15.f) : 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c[j] = nearest_whole(v[j], step, inv);
+    for (int j = 0; j < 8; ++j)
+      c[j] = kMagic + (step > 0.f ? __builtin_amdgcn_fmed3f(nearest_whole(v[j], step, inv) + p.zero, 0.f, 15.f) : 0.f);
   }
-  p.zero = step > 0.f ? fminf(p.zero, 15.f) : 0.f;
+  word = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) code[j] = (unsigned)__builtin_amdgcn_fmed3f(c[j] + p.zero, 0.f, 15.f);
+  for (int j = 0; j < 8; ++j) {
+    word = (__float_as_uint(__builtin_amdgcn_fmed3f(c[j], kMagic, kMagic + 15.f)) << (4 * place(j))) + word;
+    word -= __float_as_uint(kMagic) << (4 * place(j));         // (one constant for all eight)
+  }
   return p;
+}
+
+// Eight codes of each of eight lanes that make up eight words of values between them, turned round: code e of lane q
+// becomes code q of lane e, of the lanes' numbers (token's bit 1, sub's bit 1, token's bit 0), lane = 16 token + sub: the
+// lowest bits of the words of packed_kv.h's order.  Its own inverse.
+__device__ __forceinline__ unsigned pack_turned_round(unsigned x, int lane) {
+  auto stage = [&](unsigned other, int bit, unsigned low, int shift) {
+    const unsigned keep = bit ? ~low : low;
+    return (x & keep) | (__builtin_rotateright32(other, bit ? shift : 32 - shift) & ~keep);
+  };
+  x = stage(__shfl_xor(x, 32, kWave), lane >> 5 & 1, 0x0F0F0F0Fu, 4);
+  x = stage(__builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, true), lane >> 1 & 1, 0x00FF00FFu, 8);
+  return stage(__shfl_xor(x, 16, kWave), lane >> 4 & 1, 0x0000FFFFu, 16);
 }
 
 // How far a word of keys, and one of values, is turned.

@@ -2,12 +2,85 @@
 // attention, and back out of it.
 //
 // One launch norms and turns query and key heads (qk_prepare.hip's arithmetic), rounds keys to the
-// activation type, as a wider cache would keep them, and quantises keys and values.  Eight elements a lane, so a
-// group of 64 is eight lanes and a head 8 to 32.  A token's keys are words of their own.  Four tokens share a word
-// of values, so the first of a run of up to four that share words writes for the run, with what it leaves of other
-// tokens' bits read first; no other request has tokens in that page's block, and a step's tokens of one request are in order.
+// activation type, as a wider cache would keep them, and quantises keys and values, eight elements a lane.  A wave
+// takes a head of neighbouring tokens, for queries and keys (a token's keys are words of their own).  Four tokens share
+// words of values, so there a wave takes those of a run of up to four that share words, sixteen lanes each, and makes
+// the words between its lanes (pack_turned_round); of a run that is not whole, what the words hold of other tokens is read first; no
+// other request has tokens in that page's block, and a step's tokens of one request are in order.  Prompts: four heads a wave,
+// which its tokens' positions and pages are looked up for once.  Bound by the instructions: 120 for eight elements;.
 #include "packed_kv.h"
 #include "qk_prepare.h"
+
+// How a step's tokens and heads go round the waves: first those that take a head of 64 / lanes tokens (`rows`), then those
+// that take runs of tokens that share words of values, and units of sixteen lanes: two heads of up to 64
+// elements, one of up to 128, half of a longer one.
+constexpr int kPackHeads = 4;
+struct PackWaves {
+  unsigned rows, values;                     // waves
+  unsigned head_parts, head_parts_inv;       // waves that share a window's heads
+  unsigned unit_parts, unit_parts_inv;       // that share a window's units
+  int units, window;                         // window: tokens whose runs (by their first token) a wave takes
+};
+static int pack_lanes(int hd) { return hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
+// Steps that fill the card many times over: four heads and the runs of four tokens a wave; fewer: one, for the sake of
+// the time of one.
+static bool pack_waves(PackWaves& w, int& heads, unsigned& blocks, int64_t tokens, int row_heads, int nkv, int lanes) {
+  w.units = (nkv * lanes + 15) / 16;
+  const int64_t in_wave = kWave / lanes, windows = (tokens + in_wave - 1) / in_wave;
+  const bool many = windows * row_heads > 16384;
+  heads = many ? kPackHeads : 1, w.window = many ? 4 : 1;
+  w.head_parts = (row_heads + heads - 1) / heads, w.unit_parts = (w.units + heads - 1) / heads;
+  w.head_parts_inv = inverse32(w.head_parts), w.unit_parts_inv = inverse32(w.unit_parts);
+  const int64_t rows = windows * w.head_parts, values = (tokens + w.window - 1) / w.window * w.unit_parts;
+  if (rows + values > 2147483647LL) return false;
+  w.rows = (unsigned)rows, w.values = (unsigned)values, blocks = (unsigned)((rows + values + 3) / 4);
+  return true;
+}
+
+// The runs of a wave of the second kind, one after the other (all of it is the same in all lanes).
+struct PackRuns {
+  int token, count, entry, pos;              // the run: its first token, how many, whose, where
+  int part;                                  // which of the waves that share the window's units
+  int base, first_pos, first_entry;          // (of lane l: of token base + l)
+  unsigned firsts, left;
+  template <typename ARGS>
+  __device__ __forceinline__ PackRuns(const ARGS& a, unsigned wave) {
+    const unsigned at = divided(wave, a.waves.unit_parts, a.waves.unit_parts_inv);
+    part = (int)(wave - at * a.waves.unit_parts);
+    base = (int)at * a.waves.window;
+    const int t = base + (int)(threadIdx.x % kWave % 8), here = min(t, a.num_tokens - 1), before = max(here - 1, 0);
+    first_pos = a.positions[here], first_entry = a.entry_of_token[here];
+    const bool goes_on = t > 0 && t < a.num_tokens && (first_pos & 3) != 0 && a.entry_of_token[before] == first_entry &&
+                         a.positions[before] == first_pos - 1;
+    firsts = (unsigned)__builtin_amdgcn_ballot_w64(!goes_on) & 0xffu;
+    left = firsts & ((1u << min(a.waves.window, a.num_tokens - base)) - 1u);
+  }
+  __device__ __forceinline__ bool next() {
+    if (left == 0) return false;
+    const int c = __builtin_ctz(left);
+    left &= left - 1;
+    token = base + c;
+    count = __builtin_ctz(firsts >> (c + 1) | 8u) + 1;
+    pos = __builtin_amdgcn_readlane(first_pos, c), entry = __builtin_amdgcn_readlane(first_entry, c);
+    return true;
+  }
+};
+
+// What of a unit a lane has.
+struct PackUnit {
+  int head, sub;           // eight elements from 8 sub on
+  bool held, there;        // the head, and elements of it
+  __device__ __forceinline__ PackUnit(int u, int lanes, int lane, int hd, int nkv) {
+    const int in = lane % 16;
+    const int h = lanes == 8 ? 2 * u + in / 8 : lanes == 16 ? u : u / 2;
+    sub = lanes == 8 ? in % 8 : lanes == 16 ? in : u % 2 * 16 + in;
+    held = h < nkv, head = min(h, nkv - 1), there = held && sub * 8 < hd;
+  }
+  // The word of its block that is this lane's behind pack_turned_round; i: which of the four tokens is the lane's.
+  __device__ __forceinline__ int word(int quad, int i, int slices) const {
+    return (quad * 16 + sub % 2 * 8 + (i / 2 + sub / 2 % 2 * 2 + i % 2 * 4)) * slices + sub / 4;
+  }
+};
 
 struct PackStoreArgs {
   const void *q, *k, *v;     // rows of T: heads of a token side by side, rows `*_stride` elements apart (q: or null)
@@ -18,154 +91,142 @@ struct PackStoreArgs {
   int64_t stride;            // elements from a token's row to the next, the same in q, k and v
   int table_width, num_tokens, nq, nkv, hd, page_size;
   float eps;
-  unsigned heads, heads_inv;     // heads of a token's row (inverse32: common.h)
+  PackWaves waves;
 };
 
-// LANES: of a head (8, 16, 32), eight elements each.
-template <typename T, int LANES>
+// LANES: of a head (8, 16, 32), eight elements each; HEADS: that a wave takes one after the other.
+template <typename T, int LANES, int HEADS>
 __global__ __launch_bounds__(256) void pack_store_kernel(PackStoreArgs a) {
-  constexpr int kHeads = kWave / LANES;
-  const int lane = threadIdx.x % kWave, sub = lane % LANES;
-  const unsigned item = (blockIdx.x * 4 + threadIdx.x / kWave) * kHeads + lane / LANES;
-  const int t = (int)divided(item, a.heads, a.heads_inv), h = (int)(item - t * a.heads);
-  if (t >= a.num_tokens) return;                               // whole heads: groups of LANES lanes
-  const int hd = a.hd, pos = a.positions[t], entry = a.entry_of_token[t];
-  const bool there = sub * 8 < hd;
-  const int at = there ? sub * 8 : 0;
-  const int bytes = pack_block_bytes(hd), G = pack_groups(hd), NB = pack_slices(hd);
-  if (h < a.nq + a.nkv) {
-    const bool key = h >= a.nq;
-    const int head = key ? h - a.nq : h;
-    Eight<T> x;
-    x.load((const T*)(key ? a.k : a.q) + (int64_t)t * a.stride + (int64_t)head * hd + at);
-    float v[8];
+  const int lane = threadIdx.x % kWave;
+  const int hd = a.hd, bytes = pack_block_bytes(hd), G = pack_groups(hd), NB = pack_slices(hd);
+  unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
+  if (wave < a.waves.rows) {
+    const int sub = lane % LANES;
+    const unsigned window = divided(wave, a.waves.head_parts, a.waves.head_parts_inv);
+    const int h0 = (int)(wave - window * a.waves.head_parts) * HEADS;
+    const int token_at = (int)window * (kWave / LANES) + lane / LANES;
+    const bool in_step = token_at < a.num_tokens, there = sub * 8 < hd;
+    const int t = min(token_at, a.num_tokens - 1), at = there ? sub * 8 : 0;
+    const int pos = a.positions[t], entry = a.entry_of_token[t], last = a.nq + a.nkv - 1;
+    Eight<T> x[HEADS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = there ? x.get(j) : 0.f;
-    const float* w = key ? a.k_weight : a.q_weight;
-    if (w) {
-      const float rstd = head_rstd(v, LANES, hd, a.eps);
-      const f32x4_qk w0 = *(const f32x4_qk*)(w + at), w1 = *(const f32x4_qk*)(w + at + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { v[j] *= rstd * w0[j]; v[4 + j] *= rstd * w1[j]; }
+    for (int i = 0; i < HEADS; ++i) {
+      const int h = min(h0 + i, last);
+      x[i].load((const T*)(h >= a.nq ? a.k : a.q) + (int64_t)t * a.stride + (int64_t)(h >= a.nq ? h - a.nq : h) * hd + at);
     }
+    const int page = a.table[(int64_t)entry * a.table_width + (pos >> __builtin_ctz(a.page_size))];
+    const int half = hd / 16;                                  // lanes of half a head
+    const bool first = sub < half;
+    const int other_lane = there ? lane - sub + (first ? sub + half : sub - half) : lane;
+    f32x4_qk c0, c1, s0, s1;
     if (a.cos) {
-      const int half = hd / 16;                                // lanes of half a head
-      const bool first = sub < half;
       const int i0 = (first ? sub : there ? sub - half : 0) * 8;
       const float* cp = a.cos + (int64_t)pos * (hd / 2) + i0;
       const float* sp = a.sin + (int64_t)pos * (hd / 2) + i0;
-      const f32x4_qk c0 = *(const f32x4_qk*)cp, c1 = *(const f32x4_qk*)(cp + 4);
-      const f32x4_qk s0 = *(const f32x4_qk*)sp, s1 = *(const f32x4_qk*)(sp + 4);
-      const int other_lane = there ? lane - sub + (first ? sub + half : sub - half) : lane;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float other = __shfl(v[j], other_lane, kWave);
-        v[j] = head_turned(v[j], other, j < 4 ? c0[j] : c1[j - 4], j < 4 ? s0[j] : s1[j - 4], first);
-      }
+      c0 = *(const f32x4_qk*)cp, c1 = *(const f32x4_qk*)(cp + 4);
+      s0 = *(const f32x4_qk*)sp, s1 = *(const f32x4_qk*)(sp + 4);
     }
-    if (!key) {
-      if (there) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x.set(j, v[j]);
-        x.store((T*)a.q_out + ((int64_t)t * a.nq + head) * hd + at);
-      }
-      return;
-    }
-    const int page = a.table[(int64_t)entry * a.table_width + (pos >> __builtin_ctz(a.page_size))];
-    unsigned code[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = there ? to_f32(from_f32<T>(v[j])) : 0.f;
-    const PackGroup p = pack_eight(v, code);
-    if (page < 0) return;                                      // no page behind this position: nothing is written
     const int slot = pos & (a.page_size - 1), token = slot % kPackTokens;
-    unsigned char* block = a.k_pages + pack_block(page, a.nkv, head, a.page_size, slot, bytes);
-    unsigned word = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) word |= code[j] << (4 * (j / 2 + 4 * (j % 2)));
-    if (sub < NB * 4) ((unsigned*)block)[(sub % 4 * 16 + token) * NB + sub / 4] = pack_turned<kPackTurnK>(word);
-    if (sub % 8 == 0 && there) {
-      _Float16* scale = (_Float16*)(block + pack_codes_bytes(hd) + (token / 4 * G + sub / 8) * 16);
-      scale[token % 4] = p.step;
-      scale[4 + token % 4] = (_Float16)(-16.f - p.zero);
+    for (int i = 0; i < HEADS; ++i) {
+      const int h = h0 + i;
+      if (h > last) break;
+      const bool key = h >= a.nq;
+      const int head = key ? h - a.nq : h;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = there ? x[i].get(j) : 0.f;
+      const float* w = key ? a.k_weight : a.q_weight;
+      if (w) {
+        const float rstd = head_rstd(v, LANES, hd, a.eps);
+        const f32x4_qk w0 = *(const f32x4_qk*)(w + at), w1 = *(const f32x4_qk*)(w + at + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { v[j] *= rstd * w0[j]; v[4 + j] *= rstd * w1[j]; }
+      }
+      if (a.cos) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float other = __shfl(v[j], other_lane, kWave);
+          v[j] = head_turned(v[j], other, j < 4 ? c0[j] : c1[j - 4], j < 4 ? s0[j] : s1[j - 4], first);
+        }
+      }
+      if (!key) {
+        if (there && in_step) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[i].set(j, v[j]);
+          x[i].store((T*)a.q_out + ((int64_t)t * a.nq + head) * hd + at);
+        }
+        continue;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = there ? to_f32(from_f32<T>(v[j])) : 0.f;
+      unsigned word;
+      const PackGroup p = pack_eight(v, word, [](int j) { return j / 2 + 4 * (j % 2); });
+      if (page < 0 || !in_step) continue;                      // no page behind this position: nothing is written
+      unsigned char* block = a.k_pages + pack_block(page, a.nkv, head, a.page_size, slot, bytes);
+      if (sub < NB * 4) ((unsigned*)block)[(sub % 4 * 16 + token) * NB + sub / 4] = pack_turned<kPackTurnK>(word);
+      if (sub % 8 == 0 && there) {
+        _Float16* scale = (_Float16*)(block + pack_codes_bytes(hd) + (token / 4 * G + sub / 8) * 16);
+        scale[token % 4] = p.step;
+        scale[4 + token % 4] = (_Float16)(-16.f - p.zero);
+      }
     }
     return;
   }
-  // values: the first token of those of this step that share words with it
-  const int head = h - a.nq - a.nkv, i0 = pos & 3;
-  if (i0 != 0 && t > 0 && a.entry_of_token[t - 1] == entry && a.positions[t - 1] == pos - 1) return;
-  int count = 1;
+  wave -= a.waves.rows;
+  if (wave >= a.waves.values) return;
+  PackRuns runs(a, wave);
+  const int i = lane / 16, u0 = runs.part * HEADS;
+  while (runs.next()) {
+    const int j = i - (runs.pos & 3), t = runs.token + max(min(j, runs.count - 1), 0);
+    const bool present = j >= 0 && j < runs.count;
+    Eight<T> x[HEADS];
 #pragma unroll
-  for (int j = 1; j < 4; ++j) {
-    const int n = min(t + j, a.num_tokens - 1);
-    if (count == j && i0 + j < 4 && t + j < a.num_tokens && a.entry_of_token[n] == entry && a.positions[n] == pos + j)
-      count = j + 1;
-  }
-  const int page = a.table[(int64_t)entry * a.table_width + (pos >> __builtin_ctz(a.page_size))];
-  const int slot = pos & (a.page_size - 1), quad = slot % kPackTokens / 4, second = sub / 2 % 2;
-  Eight<T> x[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    x[j].load((const T*)a.v + (int64_t)(t + min(j, count - 1)) * a.stride + (int64_t)head * hd + at);
-  unsigned part[8] = {};
-  _Float16 step[4];
-  float zero[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float v[8];
-    unsigned code[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = there ? x[j].get(e) : 0.f;
-    const PackGroup p = pack_eight(v, code);
-    step[j] = p.step, zero[j] = p.zero;
-    const int i = (i0 + j) & 3;                                // (of tokens past the run: not used)
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (j < count) part[e] |= code[e] << (4 * (2 * second + i / 2 + 4 * (i % 2)));
-  }
-  unsigned mask = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int i = (i0 + j) & 3;
-    if (j < count) mask |= 0xfu << (4 * (i / 2 + 4 * (i % 2)));
-  }
-  mask |= mask << 8;                                           // both elements of a word
-  unsigned word[4];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const unsigned both = part[e] | __shfl_xor(part[e], 2, kWave);
-    if (e / 4 == second) word[e % 4] = both;
-  }
-  if (page < 0) return;
-  unsigned char* block = a.v_pages + pack_block(page, a.nkv, head, a.page_size, slot, bytes);
-  if (sub < NB * 4) {
-    unsigned* words = (unsigned*)block + (quad * 16 + sub % 2 * 8 + second * 4) * NB + sub / 4;
-    if (count < 4) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) word[e] |= pack_unturned<kPackTurnV>(words[e * NB]) & ~mask;
+    for (int n = 0; n < HEADS; ++n) {
+      const PackUnit u(u0 + n, LANES, lane, hd, a.nkv);
+      x[n].load((const T*)a.v + (int64_t)t * a.stride + (int64_t)u.head * hd + (u.there ? u.sub * 8 : 0));
     }
+    const int page = a.table[(int64_t)runs.entry * a.table_width + (runs.pos >> __builtin_ctz(a.page_size))];
+    const int slot = runs.pos & (a.page_size - 1), quad = slot % kPackTokens / 4;
+    unsigned mask = 0;                                         // of the run's tokens in a word
 #pragma unroll
-    for (int e = 0; e < 4; ++e) words[e * NB] = pack_turned<kPackTurnV>(word[e]);
-  }
-  if (sub % 8 == 0 && there) {
-    unsigned char* scale = block + pack_codes_bytes(hd) + (quad * G + sub / 8) * 16;
+    for (int k = 0; k < 4; ++k)
+      if (k >= (runs.pos & 3) && k < (runs.pos & 3) + runs.count) mask |= 0xf0fu << (4 * (k / 2 + 4 * (k % 2)));
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < count) {
-        ((_Float16*)scale)[i0 + j] = step[j];
-        ((_Float16*)scale)[4 + i0 + j] = (_Float16)(-16.f - zero[j]);
+    for (int n = 0; n < HEADS; ++n) {
+      if (u0 + n >= a.waves.units) break;
+      const PackUnit u(u0 + n, LANES, lane, hd, a.nkv);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = u.there ? x[n].get(e) : 0.f;
+      unsigned word;
+      const PackGroup p = pack_eight(v, word, [](int e) { return e; });
+      word = pack_turned_round(present ? word : 0u, lane);
+      if (page < 0 || !u.held) continue;
+      unsigned char* block = a.v_pages + pack_block(page, a.nkv, u.head, a.page_size, slot, bytes);
+      if (u.sub < NB * 4) {
+        unsigned* at = (unsigned*)block + u.word(quad, i, NB);
+        if (runs.count < 4) word |= pack_unturned<kPackTurnV>(*at) & ~mask;
+        *at = pack_turned<kPackTurnV>(word);
       }
+      if (u.sub % 8 == 0 && u.there && present) {
+        _Float16* scale = (_Float16*)(block + pack_codes_bytes(hd) + (quad * G + u.sub / 8) * 16);
+        scale[i] = p.step;
+        scale[4 + i] = (_Float16)(-16.f - p.zero);
+      }
+    }
   }
 }
 
 static int launch_pack_store(PackStoreArgs a, int type, hipStream_t stream) {
-  const int lanes = a.hd <= 64 ? 8 : a.hd <= 128 ? 16 : 32;
-  a.heads = a.nq + 2 * a.nkv, a.heads_inv = inverse32(a.heads);
-  const int64_t items = (int64_t)a.num_tokens * a.heads;
-  const int per_block = 4 * (kWave / lanes);
-  const int64_t blocks = (items + per_block - 1) / per_block;
-  if (items > 2147483647LL - per_block) TS_FAIL("pack_store: too many tokens");
-#define TS_LAUNCH(L) hipLaunchKernelGGL((pack_store_kernel<T, L>), dim3((unsigned)blocks), dim3(256), 0, stream, a)
-  TS_DISPATCH_TYPE(type, T, if (lanes == 8) TS_LAUNCH(8); else if (lanes == 16) TS_LAUNCH(16); else TS_LAUNCH(32));
+  const int lanes = pack_lanes(a.hd);
+  int heads;
+  unsigned blocks;
+  if (!pack_waves(a.waves, heads, blocks, a.num_tokens, a.nq + a.nkv, a.nkv, lanes)) TS_FAIL("pack_store: too many tokens");
+#define TS_LAUNCH(L) \
+  if (heads == 1) hipLaunchKernelGGL((pack_store_kernel<T, L, 1>), dim3(blocks), dim3(256), 0, stream, a); \
+  else hipLaunchKernelGGL((pack_store_kernel<T, L, kPackHeads>), dim3(blocks), dim3(256), 0, stream, a);
+  TS_DISPATCH_TYPE(type, T, if (lanes == 8) { TS_LAUNCH(8) } else if (lanes == 16) { TS_LAUNCH(16) } else { TS_LAUNCH(32) });
 #undef TS_LAUNCH
   TS_CHECK_LAUNCH("pack_store");
   return 0;
@@ -219,63 +280,81 @@ extern "C" int ts_pack_store(const void* k, const void* v, int type, void* k_pag
 }
 
 // ---------------------------------------------------------------- back out of the cache
-// Eight elements a lane of a token's key or value head; the first of up to four tokens that share words of values reads
-// for all of them.  Positions without a page read as zeros.
+// The same waves: a head of neighbouring tokens' keys, then runs that share words of values.  Positions without a page
+// read as zeros.
 struct PackValuesArgs {
   const unsigned char *k_pages, *v_pages;
   void *k, *v;                   // [T, nkv, hd]
   const int *positions, *entry_of_token, *table;
   int table_width, num_tokens, nkv, hd, page_size;
-  unsigned per, per_inv, heads_inv;      // pieces of a head; of 2 nkv
+  PackWaves waves;
 };
 
-template <typename T>
+template <typename T, int LANES, int HEADS>
 __global__ __launch_bounds__(256) void pack_values_kernel(PackValuesArgs a) {
-  const unsigned piece = blockIdx.x * 256 + threadIdx.x, row = divided(piece, a.per, a.per_inv);
-  const int sub = (int)(piece - row * a.per);
-  const int t = (int)divided(row, 2 * a.nkv, a.heads_inv), h = (int)(row - (unsigned)t * 2 * a.nkv);
-  if (t >= a.num_tokens) return;
-  const bool key = h < a.nkv;
-  const int head = key ? h : h - a.nkv, pos = a.positions[t], entry = a.entry_of_token[t];
-  int count = 1;
-  if (!key) {
-    const int i0 = pos & 3;
-    if (i0 != 0 && t > 0 && a.entry_of_token[t - 1] == entry && a.positions[t - 1] == pos - 1) return;
-#pragma unroll
-    for (int j = 1; j < 4; ++j) {
-      const int n = min(t + j, a.num_tokens - 1);
-      if (count == j && i0 + j < 4 && t + j < a.num_tokens && a.entry_of_token[n] == entry && a.positions[n] == pos + j)
-        count = j + 1;
-    }
-  }
-  const int page = a.table[(int64_t)entry * a.table_width + (pos >> __builtin_ctz(a.page_size))];
-  const int G = pack_groups(a.hd), NB = pack_slices(a.hd), slot = pos & (a.page_size - 1), token = slot % kPackTokens;
-  const int quad = token / 4, i0 = token % 4;
-  const unsigned char* block = (key ? a.k_pages : a.v_pages) +
-                               pack_block(max(page, 0), a.nkv, head, a.page_size, slot, pack_block_bytes(a.hd));
-  const unsigned* words = (const unsigned*)block;
-  typedef _Float16 eight_h __attribute__((ext_vector_type(8)));
-  const eight_h scale = *(const eight_h*)(block + pack_codes_bytes(a.hd) + (quad * G + sub / 8) * 16);
-  T* dst = (T*)(key ? a.k : a.v) + ((int64_t)t * a.nkv + head) * a.hd + sub * 8;
-  unsigned word[8];
-  if (key) {
-    word[0] = pack_unturned<kPackTurnK>(words[(sub % 4 * 16 + token) * NB + sub / 4]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) word[e] = pack_unturned<kPackTurnV>(words[(quad * 16 + sub % 2 * 8 + e) * NB + sub / 4]);
-  }
-  for (int j = 0; j < count; ++j) {
-    const int i = i0 + j;
-    const float step = page >= 0 ? (float)(i == 0 ? scale[0] : i == 1 ? scale[1] : i == 2 ? scale[2] : scale[3]) : 0.f;
-    const float bias = (float)(i == 0 ? scale[4] : i == 1 ? scale[5] : i == 2 ? scale[6] : scale[7]);
-    const int at = 4 * (2 * (sub / 2 % 2) + i / 2 + 4 * (i % 2));
+  const int lane = threadIdx.x % kWave;
+  const int hd = a.hd, bytes = pack_block_bytes(hd), G = pack_groups(hd), NB = pack_slices(hd);
+  auto put = [&](T* dst, unsigned word, float step, float bias, auto place) {
     Eight<T> out;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned code = key ? word[0] >> (4 * (e / 2 + 4 * (e % 2))) & 15 : word[e] >> at & 15;
-      out.set(e, page >= 0 ? step * ((float)code + 16.f + bias) : 0.f);
+    for (int e = 0; e < 8; ++e) out.set(e, step * ((float)(word >> (4 * place(e)) & 15u) + 16.f + bias));
+    out.store(dst);
+  };
+  unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
+  if (wave < a.waves.rows) {
+    const int sub = lane % LANES;
+    const unsigned window = divided(wave, a.waves.head_parts, a.waves.head_parts_inv);
+    const int h0 = (int)(wave - window * a.waves.head_parts) * HEADS;
+    const int t = (int)window * (kWave / LANES) + lane / LANES;
+    if (t >= a.num_tokens || sub * 8 >= hd) return;
+    const int pos = a.positions[t], entry = a.entry_of_token[t];
+    const int page = a.table[(int64_t)entry * a.table_width + (pos >> __builtin_ctz(a.page_size))];
+    const int slot = pos & (a.page_size - 1), token = slot % kPackTokens;
+    unsigned word[HEADS];
+    _Float16 step[HEADS], bias[HEADS];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+      const unsigned char* block = a.k_pages + pack_block(max(page, 0), a.nkv, min(h0 + i, a.nkv - 1), a.page_size, slot, bytes);
+      word[i] = ((const unsigned*)block)[(sub % 4 * 16 + token) * NB + sub / 4];
+      const _Float16* scale = (const _Float16*)(block + pack_codes_bytes(hd) + (token / 4 * G + sub / 8) * 16) + token % 4;
+      step[i] = scale[0], bias[i] = scale[4];
     }
-    out.store(dst + (int64_t)j * a.nkv * a.hd);
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i)
+      if (h0 + i < a.nkv)
+        put((T*)a.k + ((int64_t)t * a.nkv + h0 + i) * hd + sub * 8, pack_unturned<kPackTurnK>(word[i]),
+            page >= 0 ? (float)step[i] : 0.f, page >= 0 ? (float)bias[i] : 0.f, [](int j) { return j / 2 + 4 * (j % 2); });
+    return;
+  }
+  wave -= a.waves.rows;
+  if (wave >= a.waves.values) return;
+  PackRuns runs(a, wave);
+  const int i = lane / 16, u0 = runs.part * HEADS;
+  while (runs.next()) {
+    const int j = i - (runs.pos & 3), t = runs.token + max(min(j, runs.count - 1), 0);
+    const bool present = j >= 0 && j < runs.count;
+    const int page = a.table[(int64_t)runs.entry * a.table_width + (runs.pos >> __builtin_ctz(a.page_size))];
+    const int slot = runs.pos & (a.page_size - 1), quad = slot % kPackTokens / 4;
+    unsigned word[HEADS];
+    _Float16 step[HEADS], bias[HEADS];
+#pragma unroll
+    for (int n = 0; n < HEADS; ++n) {
+      const PackUnit u(min(u0 + n, a.waves.units - 1), LANES, lane, hd, a.nkv);
+      const int sub = u.there ? u.sub : 0;                     // (a lane behind the head's end: of no consequence)
+      const unsigned char* block = a.v_pages + pack_block(max(page, 0), a.nkv, u.head, a.page_size, slot, bytes);
+      word[n] = u.sub < NB * 4 ? ((const unsigned*)block)[u.word(quad, i, NB)] : 0u;
+      const _Float16* scale = (const _Float16*)(block + pack_codes_bytes(hd) + (quad * G + sub / 8) * 16) + i;
+      step[n] = scale[0], bias[n] = scale[4];
+    }
+#pragma unroll
+    for (int n = 0; n < HEADS; ++n) {
+      if (u0 + n >= a.waves.units) break;
+      const PackUnit u(u0 + n, LANES, lane, hd, a.nkv);
+      const unsigned own = pack_turned_round(pack_unturned<kPackTurnV>(word[n]), lane);
+      if (present && u.there)
+        put((T*)a.v + ((int64_t)t * a.nkv + u.head) * hd + u.sub * 8, own, page >= 0 ? (float)step[n] : 0.f,
+            page >= 0 ? (float)bias[n] : 0.f, [](int e) { return e; });
+    }
   }
 }
 
@@ -287,13 +366,17 @@ extern "C" int ts_pack_values(const void* k_pages, const void* v_pages, void* k,
   if (nkv <= 0 || !table || table_width <= 0) TS_FAIL("pack_values: nkv=%d, block table of width %d", nkv, table_width);
   if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15)
     TS_FAIL("pack_values: tensors must be 16-byte aligned");
-  const int64_t pieces = (int64_t)num_tokens * 2 * nkv * (hd / 8), blocks = (pieces + 255) / 256;
-  if (pieces > 2147483647LL - 256) TS_FAIL("pack_values: too many tokens");
-  const unsigned per = hd / 8, heads = 2 * nkv;
-  const PackValuesArgs a{(const unsigned char*)k_pages, (const unsigned char*)v_pages, k, v, positions, entry_of_token,
-                         table, table_width, num_tokens, nkv, hd, page_size, per, inverse32(per), inverse32(heads)};
-  TS_DISPATCH_TYPE(type, T,
-      hipLaunchKernelGGL(pack_values_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream, a));
+  const int lanes = pack_lanes(hd);
+  PackValuesArgs a{(const unsigned char*)k_pages, (const unsigned char*)v_pages, k, v, positions, entry_of_token,
+                   table, table_width, num_tokens, nkv, hd, page_size, {}};
+  int heads;
+  unsigned blocks;
+  if (!pack_waves(a.waves, heads, blocks, num_tokens, nkv, nkv, lanes)) TS_FAIL("pack_values: too many tokens");
+#define TS_LAUNCH(L) \
+  if (heads == 1) hipLaunchKernelGGL((pack_values_kernel<T, L, 1>), dim3(blocks), dim3(256), 0, stream, a); \
+  else hipLaunchKernelGGL((pack_values_kernel<T, L, kPackHeads>), dim3(blocks), dim3(256), 0, stream, a);
+  TS_DISPATCH_TYPE(type, T, if (lanes == 8) { TS_LAUNCH(8) } else if (lanes == 16) { TS_LAUNCH(16) } else { TS_LAUNCH(32) });
+#undef TS_LAUNCH
   TS_CHECK_LAUNCH("pack_values");
   return 0;
 }
