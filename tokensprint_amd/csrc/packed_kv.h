@@ -66,7 +66,7 @@ struct PackGroup {
 
 // The group of the eight lanes that hold 64 elements between them, eight each (`v`; elements that are not there are
 // zeros), and this lane's codes, in the order that `place` gives: element j's in bits 4 place(j) on.  A quotient by the
-// estimate of 1 / step is off by less than 2^-18, so a code is the whole number next to it (which adding 1.5 x 2^23 leaves in
+// estimate of 1 / step is off by less than 2^-17 (two roundings of at most 15), so a code is the whole number next to it (which adding 1.5 x 2^23 leaves in
 // the lowest bits) unless that is nearly half a step away; where one of a wavefront's is, all are worked out with what
 // is left over (exactly: ties to even), and where one is no finite number, they are made one.
 template <typename PLACE>
@@ -98,7 +98,9 @@ __device__ __forceinline__ PackGroup pack_eight(float (&v)[8], unsigned& word, P
     range();
   }
   PackGroup p;
-  p.step = (_Float16)fminf((hi - lo) / 15.f, 65504.f);
+  // (hi - lo) / 15, rounded as a division rounds it (checked for every significand); of an infinite range NaN, so the most
+  const float wide = hi - lo, about = wide * (1.f / 15.f);
+  p.step = (_Float16)fminf(fmaf(fmaf(-15.f, about, wide), 1.f / 15.f, about), 65504.f);
   const float step = (float)p.step, inv = step > 0.f ? __builtin_amdgcn_rcpf(step) : 0.f;
   p.zero = rintf(-lo * inv);
   float off = fabsf(fmaf(-lo, inv, -p.zero)), c[8];
@@ -109,7 +111,7 @@ __device__ __forceinline__ PackGroup pack_eight(float (&v)[8], unsigned& word, P
     c[j] = fmaf(v[j], inv, one);
     off = fmaxf(off, fabsf(fmaf(v[j], inv, one - c[j])));
   }
-  if (__builtin_amdgcn_ballot_w64(off > 0.4999f || step >= 65504.f) != 0) {
+  if (__builtin_amdgcn_ballot_w64(off > 0.49999f || step >= 65504.f) != 0) {
     p.zero = nearest_whole(-lo, step, inv);
     p.zero = step > 0.f ? fminf(p.zero, 15.f) : 0.f;
 #pragma unroll
