@@ -243,3 +243,35 @@ def test_rows_of_tiny_elements(ops, rows, k, top):
     assert ((scale - x.double().abs().amax(1) / 127).abs() <= scale * 2.0**-24 + 2.0**-150).all()
     ratio = x.double() / scale[:, None]
     assert ((got.codes.cpu()[:, :k].double() - ratio.clamp(-127, 127)).abs() <= 0.5).all()
+
+
+@pytest.mark.parametrize("k", [8, 264, 2816, 4096, 8192, 8200])
+@pytest.mark.parametrize("rows", [1, 2, 4, 5])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_call_is_the_two_calls_to_the_bit(ops, rows, k, dtype):
+    torch.manual_seed(k + rows)
+    weight = ops.quantize_weight(torch.randn(2 * 77, k, device="cuda"))
+    x = torch.randn(rows, k, device="cuda").to(dtype)
+    assert torch.equal(ops.linear(x, weight, dtype), ops.linear(ops.quantize_rows(x), weight, dtype))
+    assert torch.equal(ops.linear_silu_mul(x, weight, dtype),
+                       ops.linear_silu_mul(ops.quantize_rows(x), weight, dtype))
+    stream, w = torch.randn(rows, k, device="cuda"), torch.rand(k, device="cuda")
+    for delta in (x, None):
+        for pair in (False, True):
+            before = stream.clone()
+            out, after = ops.norm_linear(stream, delta, w, 1e-6, weight, dtype, silu_mul=pair)
+            normed, want = ops.norm_quantize_rows(stream, delta, w, 1e-6)
+            assert torch.equal(out, (ops.linear_silu_mul if pair else ops.linear)(normed, weight, dtype))
+            assert torch.equal(after, want) and torch.equal(stream, before)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_one_call_with_a_row_that_is_not_finite(ops, value):
+    """The other rows know nothing of it."""
+    weight = ops.quantize_weight(torch.randn(48, 512, device="cuda"))
+    x = torch.randn(3, 512, device="cuda")
+    want = ops.linear(x, weight, torch.float32)
+    x[1, 300] = value
+    got = ops.linear(x, weight, torch.float32)
+    assert torch.equal(got[[0, 2]], want[[0, 2]])
+    assert not torch.isfinite(got[1]).any()
