@@ -21,9 +21,7 @@ int ts_check_packed_args(const PackedArgs& args, const char* who) {
 }
 
 // Workgroups of the kernel that shares keys out which the card holds at a time.
-extern "C" int ts_packed_resident(int hd, int type) {
-  return compute_units() * packed_waves(pack_slices(hd), type == TS_F32);
-}
+extern "C" int ts_packed_resident() { return compute_units(); }
 
 // `coop`: all items' keys shared out over `workgroups` workgroups, else a wavefront per item.
 extern "C" int ts_packed_attention(const PackedArgs* p, int type, int coop, hipStream_t stream) {

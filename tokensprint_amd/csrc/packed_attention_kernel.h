@@ -359,13 +359,12 @@ __device__ __forceinline__ void packed_finish(PackedTile<NB, WIDE>& t) {
 // Workgroups of four wavefronts that a compute unit holds, by the registers they take.
 __host__ __device__ constexpr int packed_waves(int nb, bool wide) { return nb > 4 ? (wide ? 1 : 2) : wide ? 2 : 3; }
 
-constexpr int kPackedChunk = 128;      // keys: a block for each of a workgroup's wavefronts
-
 // One tile's query rows and how far they see.
 struct PackedItem {
   int entry, tok0, ntok, pos_first, pos_last;
   KeyWalk walk;
-  __device__ __forceinline__ int chunks() const { return (pos_last - walk.origin) / kPackedChunk + 1; }
+  template <int TURN>
+  __device__ __forceinline__ int chunks() const { return (pos_last - walk.origin) / TURN + 1; }
 };
 __device__ __forceinline__ PackedItem packed_item(const PackedArgs& args, int tile) {
   PackedItem it;
@@ -401,21 +400,94 @@ __device__ __forceinline__ int lanes_before(int v, int lane) {
   return v;
 }
 
-// An item is a tile and a key/value head (and a block of 16 of its query heads); the chunks of 128 keys of
-// all items, one behind the other, are shared out evenly: every workgroup walks as many, whatever the lengths of the
-// requests, of one item or of several.  The lengths are on the device only (a captured step's), so every wavefront adds
-// them up for itself.  (A workgroup per item and share of at most 2,048 keys: 64 requests of 128 to 4,096 tokens 50 us, the chip
-// half empty behind the longest.)
-// A workgroup's four wavefronts take every fourth block of 32 keys and merge in LDS.  An item that ends in another
-// workgroup than it began in leaves its parts in memory, two places a workgroup (the part that an earlier one began, the
-// part that a later one goes on with), and whoever comes last merges them in their order.
-template <int NB, bool WIDE, bool EXTRA, typename T>
-__global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_kernel(PackedArgs args) {
+// What is a workgroup's of all items, by one of its wavefronts: turns `at` .. `end` of all, the tile in which they begin and
+// its first turn, and how many turns a workgroup has where they are shared.
+template <int TURN>
+__device__ __forceinline__ void packed_plan(const PackedArgs& args, int heads, int lane, int (&plan)[5]) {
+  const int last = kWave - 1, index = blockIdx.x, items = args.num_tiles * heads;
+  int total = 0, most = 0, n = 0, upto = 0;
+  for (int t0 = 0; t0 < args.num_tiles; t0 += kWave) {
+    n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).template chunks<TURN>() : 0;
+    upto = lanes_before(n, lane);
+    total += __builtin_amdgcn_readlane(upto, last);
+    most = max(most, n);
+  }
+  most = uniform((int)wave_max((float)most));
+  const int len = (total * heads + args.workgroups - 1) / args.workgroups;
+  // in half turns (1.1 us): whole, the longest item, or, of more items than run at a time, all of them and half the
+  // longest behind; shared, a workgroup's turns, the look, the parts and their merge, and the ends of items on the way
+  const bool in_turns = items > args.workgroups;
+  const int whole_cost = max(2 * most, in_turns ? 2 * len + most : 0);
+  const int shared_cost = 2 * len + 7 + 12 * items / args.workgroups;
+  int at = 0, end = 0, tile = 0, tile_at = 0;
+  if (whole_cost <= shared_cost) {
+    if (index < items) {
+      tile = index / heads;
+      const int head_of = index - tile * heads;
+      if (in_turns && args.num_tiles <= kWave && most * args.num_tiles > total + total / 4) {
+        // the longest first (64 requests of 128 to 4,096 tokens: 43 us in place of 47)
+        const int mine = n * kWave + lane;
+        int longer = 0;
+        for (int j = 0; j < args.num_tiles; ++j) longer += __builtin_amdgcn_readlane(mine, j) > mine ? 1 : 0;
+        tile = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < args.num_tiles && longer == tile));
+      }
+      const int turns = packed_item_of(args, tile).template chunks<TURN>();
+      at = head_of * turns, end = at + turns;
+    }
+  } else if (index < args.workgroups && index * len < total * heads) {
+    at = index * len;
+    end = min(at + len, total * heads);
+    for (int t0 = 0, sum = 0; t0 < args.num_tiles; t0 += kWave) {
+      if (args.num_tiles > kWave) {
+        n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).template chunks<TURN>() : 0;
+        upto = sum + lanes_before(n, lane);
+      }
+      const unsigned long long here = __builtin_amdgcn_ballot_w64(upto * heads > at);
+      if (here != 0) {
+        const int l = __builtin_ctzll(here);
+        tile = t0 + l;
+        tile_at = __builtin_amdgcn_readlane(upto - n, l) * heads;
+        break;
+      }
+      sum = __builtin_amdgcn_readlane(upto, last);
+    }
+  }
+  if (lane == 0) plan[0] = at, plan[1] = end, plan[2] = tile, plan[3] = tile_at, plan[4] = len;
+}
+
+// An item is a tile and a key/value head (and a block of 16 of its query heads).  A workgroup of as many wavefronts as a
+// compute unit holds takes 32 keys a wavefront at a time, a turn of 384 with heads of up to 128, and merges its
+// wavefronts in LDS.  (Workgroups of four wavefronts, three to a unit, have three times the items' starts and ends and parts:
+// 64 requests of 4,000 tokens, 8 heads of 128, took 68 us, 5.0 TB/s and 60 us so.)
+//
+// SHARED: how far the items reach is on the device only (a captured step's), so every workgroup looks: either an item is
+// one workgroup's, or the turns of all items, one behind the other, are shared out evenly, whatever the lengths, where the
+// estimates below say that this is sooner (1 request of 8,000 tokens 46 us whole and 14 shared, 16 of 1,300 12 and 15).
+// An item that ends in another workgroup than it began in leaves its parts in memory, two places a workgroup (the part
+// that an earlier one began, the part that a later one goes on with), and whoever comes last merges them in their order, sixteen
+// parts asked for at a time (four: 25 us in place of 18 for that request).
+//
+// Not SHARED: an item a workgroup, without that look (1 us).
+template <int NB, bool WIDE>
+struct PackedShape {
+  static constexpr int WAVES = 4 * packed_waves(NB, WIDE), THREADS = WAVES * kWave;
+  static constexpr int ROW = 32 * NB + 4;                     // floats: neighbouring rows start four banks apart
+  static constexpr int LDS = WAVES * 16 * (ROW + 2) * 4;
+  static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
+};
+template <int NB, bool WIDE, bool EXTRA, typename T, bool SHARED>
+__global__ __launch_bounds__((PackedShape<NB, WIDE>::THREADS), packed_waves(NB, WIDE)) void packed_attention_kernel(
+    PackedArgs args) {
   constexpr int HD = 32 * NB, DB = 2 * NB;
-  constexpr int kRow = HD + 4;                                // neighbouring rows start four banks apart
-  __shared__ float s_ml[4][16][2];
-  __shared__ __attribute__((aligned(16))) float s_o[4][16][kRow];
+  typedef PackedShape<NB, WIDE> Shape;
+  constexpr int WAVES = Shape::WAVES, TURN = 32 * WAVES;      // TURN: keys that the workgroup takes at a time
+  extern __shared__ __attribute__((aligned(16))) float packed_lds[];
+  typedef float Results[16][Shape::ROW];
+  typedef float Stats[16][2];
+  Results* s_o = (Results*)packed_lds;
+  Stats* s_ml = (Stats*)(packed_lds + WAVES * 16 * Shape::ROW);
   __shared__ unsigned s_before[2];
+  __shared__ int s_plan[5];
   const AttentionArgs& a = args.base;
   const int wave = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int r = lane % 16, g = lane / 16;
@@ -424,34 +496,16 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_
   T* out = (T*)a.out;
 
   // this workgroup's chunks [at, end) of all, and the tile in which they begin
-  int at, end, len = 0, tile = 0, tile_at = 0;                // tile_at: the tile's first chunk among all
-  if (args.workgroups == 0) {
+  int at = 0, end = 0, len = 0, tile = 0, tile_at = 0;                // tile_at: the tile's first chunk among all
+  if constexpr (!SHARED) {
     tile = blockIdx.x / heads;
-    const int chunks = packed_item_of(args, tile).chunks();
+    const int chunks = packed_item_of(args, tile).template chunks<TURN>();
     at = (blockIdx.x - tile * heads) * chunks;
     end = at + chunks;
   } else {
-    int total = 0;
-    for (int t0 = 0; t0 < args.num_tiles; t0 += kWave) {
-      const int n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).chunks() * heads : 0;
-      total += uniform(__shfl(lanes_before(n, lane), kWave - 1, kWave));
-    }
-    len = (total + args.workgroups - 1) / args.workgroups;
-    at = blockIdx.x * len;
-    end = min(at + len, total);
-    if (at >= end) return;
-    for (int t0 = 0, sum = 0; t0 < args.num_tiles; t0 += kWave) {
-      const int n = t0 + lane < args.num_tiles ? packed_item(args, t0 + lane).chunks() * heads : 0;
-      const int upto = sum + lanes_before(n, lane);
-      const unsigned long long here = __builtin_amdgcn_ballot_w64(upto > at);
-      if (here != 0) {
-        const int l = __builtin_ctzll(here);
-        tile = t0 + l;
-        tile_at = uniform(__shfl(upto - n, l, kWave));
-        break;
-      }
-      sum = uniform(__shfl(upto, kWave - 1, kWave));
-    }
+    if (wave == 0) packed_plan<TURN>(args, heads, lane, s_plan);
+    __syncthreads();
+    at = uniform(s_plan[0]), end = uniform(s_plan[1]), tile = uniform(s_plan[2]), tile_at = uniform(s_plan[3]), len = uniform(s_plan[4]);
   }
   // the parts that this workgroup leaves in memory, one that an earlier one began and one that a later one goes on with
   struct Part {
@@ -461,7 +515,7 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_
 
   while (at < end) {
     const PackedItem it = packed_item_of(args, uniform(tile));
-    const int chunks = it.chunks(), head_of = (at - tile_at) / chunks, first_chunk = at - tile_at - head_of * chunks;
+    const int chunks = it.template chunks<TURN>(), head_of = (at - tile_at) / chunks, first_chunk = at - tile_at - head_of * chunks;
     const int count = min(chunks - first_chunk, end - at);
     const int item_at = at - first_chunk, item = tile * heads + head_of;
     const int hb = head_of % args.head_blocks, kvh = head_of / args.head_blocks;
@@ -473,12 +527,12 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_
     const int hh = hb * 16 + r % args.rows_per_token;        // head inside the group
     const bool row_ok = ti < it.ntok && hh < group;
     const int token = it.tok0 + min(ti, it.ntok - 1), head = kvh * group + min(hh, group - 1);
-    const int key_begin = it.walk.origin + first_chunk * kPackedChunk + wave * 32;
-    const int key_end = min(it.walk.origin + (first_chunk + count) * kPackedChunk, it.pos_last + 1);
+    const int key_begin = it.walk.origin + first_chunk * TURN + wave * 32;
+    const int key_end = min(it.walk.origin + (first_chunk + count) * TURN, it.pos_last + 1);
     PageCursor cur{(ConstTable)table, a.page_size, it.pos_last, it.walk, -1, -1};
     cur.start(key_begin);
     PackedBlock<NB> A, B;
-    load_packed<NB, WIDE>(A, a, cur, kvh, key_begin, kPackedChunk, lane);
+    load_packed<NB, WIDE>(A, a, cur, kvh, key_begin, TURN, lane);
     PackedTile<NB, WIDE> t;
     t.pos = row_ok ? it.pos_first + ti : -1;
     t.lo = first_visible(a, t.pos);
@@ -491,8 +545,8 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_
       const int kb = it.walk.real(v);
       packed_update<NB, WIDE, EXTRA>(t, b, kb, scale_log2, kb + 31 <= it.pos_first && kb >= lo_last, g, &x);
     };
-    for (int v = key_begin; v < key_end; v += kPackedChunk) {
-      load_packed<NB, WIDE>(B, a, cur, kvh, v + kPackedChunk, kPackedChunk, lane);
+    for (int v = key_begin; v < key_end; v += TURN) {
+      load_packed<NB, WIDE>(B, a, cur, kvh, v + TURN, TURN, lane);
       update(A, v);
       A = B;
     }
@@ -507,24 +561,24 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_
     for (int db = 0; db < DB; ++db) *(f32x4*)&s_o[wave][r][db * 16 + g * 4] = t.o[db];
     __syncthreads();
     const int rows = it.ntok * args.rows_per_token;
-    const bool whole = count == chunks;
+    const bool whole = !SHARED || count == chunks;
     const int64_t slot0 = ((int64_t)blockIdx.x * 2 + (first_chunk == 0 ? 1 : 0)) * 16;
     auto place = [&](int row) -> int64_t {                    // of a row's result, or -1: no such head
       const int rt = row / args.rows_per_token, rh = hb * 16 + row % args.rows_per_token;
       return rh < group ? ((int64_t)(it.tok0 + rt) * a.nq + kvh * group + rh) * a.hd : -1;
     };
     auto sink_of = [&](int row) { return kvh * group + hb * 16 + row % args.rows_per_token; };
-    for (int e = threadIdx.x; e < rows * HD; e += 256) {
+    for (int e = threadIdx.x; e < rows * HD; e += Shape::THREADS) {
       const int row = e / HD, d = e % HD;
       const int64_t to = place(row);
       if (to < 0 || d >= a.hd) continue;
       float M = s_ml[0][row][0];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) M = fmaxf(M, s_ml[w][row][0]);
+      for (int w = 1; w < WAVES; ++w) M = fmaxf(M, s_ml[w][row][0]);
       const float Mc = M == -INFINITY ? 0.f : M;              // (no key: all weights are 0)
       float acc = 0.f, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         const float ww = __builtin_amdgcn_exp2f(s_ml[w][row][0] - Mc);
         sum = fmaf(s_ml[w][row][1], ww, sum);
         acc = fmaf(s_o[w][row][d], ww, acc);
@@ -547,7 +601,7 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_
     }
     if (at < end) __syncthreads();                            // everybody has read what stands in LDS
   }
-  if (left == 0) return;
+  if (!SHARED || left == 0) return;
 
   // The parts' results pass the caches that another XCD does not share; each wave waits until its own have
   // been taken, the workgroup counts itself in for both, and the one that finds all others there merges.
@@ -563,15 +617,16 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_
     if ((int)s_before[which] + 1 != p.parts) continue;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
     if (threadIdx.x == 0) __hip_atomic_store(args.arrivals + p.item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int e = threadIdx.x; e < p.rows * HD; e += 256) {
+    for (int e = threadIdx.x; e < p.rows * HD; e += Shape::THREADS) {
       const int row = e / HD, d = e % HD;
       const int rt = row / args.rows_per_token, rh = p.hb * 16 + row % args.rows_per_token;
       if (rh >= group || d >= a.hd) continue;
       float M = -INFINITY, sum = 0.f, acc = 0.f;
-      for (int s0 = 0; s0 < p.parts; s0 += 4) {               // four at a time: everything asked for before its use
-        float ms[4], ls[4], po[4];
+      constexpr int AT_ONCE = 16;
+      for (int s0 = 0; s0 < p.parts; s0 += AT_ONCE) {               // everything asked for before its use
+        float ms[AT_ONCE], ls[AT_ONCE], po[AT_ONCE];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < AT_ONCE; ++j) {
           const int n = min(s0 + j, p.parts - 1);
           const int64_t slot = ((int64_t)(p.first_wg + n) * 2 + (n == 0 ? 1 : 0)) * 16 + row;
           const uint64_t ml = __hip_atomic_load((const uint64_t*)args.partial_ml + slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -581,12 +636,12 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_attention_
         }
         float Mg = M;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) Mg = fmaxf(Mg, ms[j]);
+        for (int j = 0; j < AT_ONCE; ++j) Mg = fmaxf(Mg, ms[j]);
         const float Mc = Mg == -INFINITY ? 0.f : Mg, keep = __builtin_amdgcn_exp2f(M - Mc);
         sum *= keep;
         acc *= keep;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < AT_ONCE; ++j) {
           const float w = __builtin_amdgcn_exp2f(ms[j] - Mc);
           sum = fmaf(ls[j], w, sum);
           acc = fmaf(po[j], w, acc);
@@ -651,11 +706,33 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_walk_kerne
   }
 }
 
+template <int NB, bool WIDE, bool EXTRA, typename T, bool SHARED>
+static int launch_packed_shape(const PackedArgs& args, int workgroups, hipStream_t stream) {
+  typedef PackedShape<NB, WIDE> Shape;
+  auto kernel = packed_attention_kernel<NB, WIDE, EXTRA, T, SHARED>;
+  if (Shape::LDS > 64 * 1024) {
+    static bool raised[64] = {};               // per instantiation and device
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64)
+      TS_FAIL("packed_attention: no current device below 64");
+    if (!raised[device]) {
+      if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, Shape::LDS) != hipSuccess)
+        TS_FAIL("packed_attention: cannot raise the LDS limit to %d bytes", Shape::LDS);
+      raised[device] = true;
+    }
+  }
+  hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(Shape::THREADS), Shape::LDS, stream, args);
+  TS_CHECK_LAUNCH("packed_attention");
+  return 0;
+}
+
 template <int NB, bool WIDE, bool EXTRA, typename T>
 static int launch_packed(const PackedArgs& args, bool coop, hipStream_t stream) {
   const int items = args.num_tiles * args.base.nkv * args.head_blocks;
-  if (coop)
-    hipLaunchKernelGGL((packed_attention_kernel<NB, WIDE, EXTRA, T>), dim3(args.workgroups ? args.workgroups : items), dim3(256), 0, stream, args);
+  if (coop && args.workgroups)
+    return launch_packed_shape<NB, WIDE, EXTRA, T, true>(args, items > args.workgroups ? items : args.workgroups, stream);
+  else if (coop)
+    return launch_packed_shape<NB, WIDE, EXTRA, T, false>(args, items, stream);
   else
     hipLaunchKernelGGL((packed_walk_kernel<NB, WIDE, EXTRA, T>), dim3((items + 3) / 4), dim3(256), 0, stream, args);
   TS_CHECK_LAUNCH("packed_attention");

@@ -159,7 +159,8 @@ class Dispatch:
     packed_portion: int = 16
     packed_items: int = 2048
     packed_workgroups: int = 0
-    packed_whole: int = 10
+    packed_whole: int = 1280
+    packed_whole_many: int = 4096
 
     # ---- recurrences.  A step whose longest portion has more tokens than this runs in chunks of
     # 64 tokens as products of matrices, below it every entry is walked whole by one launch.

@@ -1245,7 +1245,7 @@ class HipOps:
         if found is None:
             found = self._kept_routes()[key] = (
                 dtype is torch.bfloat16 and self.lib.ts_packed_prompt_fits(a.hd) == 1,
-                d.packed_workgroups or self.lib.ts_packed_resident(a.hd, _TYPE_CODE[dtype]))
+                d.packed_workgroups or self.lib.ts_packed_resident())
         tall, resident = found
         for portions in (True, False):
             count, tiles = self._packed_tiles(batch, portions, 8 * tokens if portions and tall else tokens,
@@ -1262,10 +1262,8 @@ class HipOps:
             if shared:
                 reach = self._reach(a)
                 keys = batch.max_ctx_len if reach == 0 else min(batch.max_ctx_len, reach + batch.max_q_len + 64)
-                chunks = -(-keys // 128)
-                if chunks > d.packed_whole:
-                    # a workgroup for every 128 keys that there can be, as many as the card holds at a time
-                    workgroups = m.workgroups = min(items * chunks, resident)
+                if keys > (d.packed_whole if items < 4 * self._units else d.packed_whole_many):
+                    workgroups = m.workgroups = resident
                     hd = -(-a.hd // 32) * 32
                     partial = torch.empty(workgroups * 32 * (hd + 2), dtype=torch.float32, device=self.device)
                     m.partial_o = at = partial.data_ptr()
