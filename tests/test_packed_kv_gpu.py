@@ -274,14 +274,17 @@ LONG = {"one": [(0, 700)], "behind": [(333, 400), (0, 65), (1, 16)], "beside": [
 @pytest.mark.parametrize("nq,nkv,hd,page", [(8, 4, 128, 16), (4, 1, 64, 32), (6, 2, 128, 64), (20, 1, 64, 16), (3, 3, 128, 256),
                                             (4, 2, 96, 16)])
 @pytest.mark.parametrize("window", [None, 100])
-def test_portions_of_prompts(ops, gpu_device, spans, nq, nkv, hd, page, window):
+def test_portions_of_prompts(ops, gpu_device, dispatch, spans, nq, nkv, hd, page, window):
+    dispatch(packed_few=0)
     check_attention(ops, gpu_device, nq=nq, nkv=nkv, hd=hd, page=page, spans=LONG[spans], dtype=torch.bfloat16,
                     window=window)
 
 
 @pytest.mark.parametrize("scale", [1e-30, 1e-4, 1e4, 1e30])
-def test_queries_of_any_magnitude(ops, gpu_device, scale):
+@pytest.mark.parametrize("few", [0, 512])
+def test_queries_of_any_magnitude(ops, gpu_device, dispatch, scale, few):
     """A row of queries is brought to float16's range: whatever it was, and rows of zeros."""
+    dispatch(packed_few=few)
     nq, nkv, hd = 4, 2, 64
     batch, whole, table, cache = scene(gpu_device, nkv=nkv, hd=hd, page=16, spans=[(30, 40), (50, 1)])
     k, v = heads_of(whole, nkv, hd, torch.bfloat16, gpu_device, 3)
@@ -331,7 +334,7 @@ OPTIONS = {
 @pytest.mark.parametrize("walk", ["shares", "one workgroup", "whole items", "wavefronts", "portions"])
 def test_attention_options(ops, gpu_device, dispatch, dtype, spans, options, walk):
     dispatch(packed_portion=1 if walk == "portions" else 1 << 20, packed_items=0 if walk == "wavefronts" else 1 << 20, packed_whole=1 << 20 if walk == "whole items" else 0,
-             packed_workgroups={"shares": 0, "one workgroup": 1}.get(walk, 7))
+             packed_workgroups={"shares": 0, "one workgroup": 1}.get(walk, 7), packed_few=0 if walk == "portions" else 512)
     kw = dict(OPTIONS[options])
     nq, nkv, hd = 6, 2, 64
     if kw.get("sink"):
@@ -352,6 +355,58 @@ def test_long_contexts_in_shares(ops, gpu_device, dispatch, dtype):
         twice = check_attention(ops, gpu_device, nq=4, nkv=2, hd=64, page=16, spans=spans, dtype=dtype)
         assert torch.equal(again, twice)             # the order of arrival changes nothing
         torch.testing.assert_close(again.float(), got.float(), rtol=2e-2, atol=2e-2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("options", list(OPTIONS))
+def test_options_in_shares(ops, gpu_device, dispatch, dtype, options):
+    """Long enough that items are shared: their parts meet what masks and scores add to them."""
+    dispatch(packed_whole=0)
+    kw = dict(OPTIONS[options])
+    if kw.get("sink"):
+        kw["sink"] = rand((6,), torch.float32, gpu_device, 31)
+    if kw.get("slopes"):
+        kw["slopes"] = torch.rand(6, device=gpu_device) * 0.01
+    check_attention(ops, gpu_device, nq=6, nkv=2, hd=64, page=16, spans=[(2600, 1), (3, 1), (900, 1)], dtype=dtype, **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nkv,spans", [
+    (8, [(37 * i * i % 1400, 1) for i in range(40)]),               # more items than units: the longest first
+    (1, [(3000 if i == 70 else i, 1) for i in range(100)]),         # more tiles than lanes, one of them shared
+    (8, [(2500 if i == 3 else 40, 1) for i in range(33)]),          # one outlier among items that take turns
+    (2, [(2000, 30), (5, 1), (0, 40), (700, 3)]),                   # portions of prompts in shares
+])
+def test_unlike_requests(ops, gpu_device, dispatch, dtype, nkv, spans):
+    whole = check_attention(ops, gpu_device, nq=2 * nkv, nkv=nkv, hd=64, page=16, spans=spans, dtype=dtype)
+    dispatch(packed_whole=0, packed_whole_many=0)
+    again = check_attention(ops, gpu_device, nq=2 * nkv, nkv=nkv, hd=64, page=16, spans=spans, dtype=dtype)
+    torch.testing.assert_close(again.float(), whole.float(), rtol=2e-2, atol=2e-2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nkv,hd", [(9, 128), (17, 64), (5, 256)])
+def test_a_long_step_is_many_short_ones(ops, gpu_device, dtype, nkv, hd):
+    """Steps of many tokens go round the waves otherwise: the same bytes, and the same numbers back."""
+    spans = [(3, 4001), (0, 1), (18, 3), (1, 2222), (6, 1900)]
+    batch, whole, table, cache = scene(gpu_device, nkv=nkv, hd=hd, page=32, spans=spans)
+    k, v = heads_of(batch, nkv, hd, dtype, gpu_device, 5)
+    other = type(cache)(**{**vars(cache), "k_pages": cache.k_pages.clone(), "v_pages": cache.v_pages.clone()})
+    ops.kv_store(k, v, batch, table, cache)
+    first = 0
+    for e, (start, n) in enumerate(spans):
+        for lo in range(0, n, 333):
+            hi = min(lo + 333, n)
+            row = table[e:e + 1].contiguous()
+            ops.kv_store(k[first + lo:first + hi], v[first + lo:first + hi],
+                         whole_batch(gpu_device, [start + hi], row, [start + lo]), row, other)
+        first += n
+    assert torch.equal(cache.k_pages, other.k_pages) and torch.equal(cache.v_pages, other.v_pages)
+    got = ops.kv_values(batch, table, cache, num_kv_heads=nkv, head_dim=hd, out_dtype=torch.float32)
+    assert torch.equal(got[0].double().cpu(), quantize4(k).cpu()) and torch.equal(got[1].double().cpu(), quantize4(v).cpu())
+    part = whole_batch(gpu_device, [spans[0][0] + 200], table[:1].contiguous(), [spans[0][0]])
+    few = ops.kv_values(part, table[:1].contiguous(), cache, num_kv_heads=nkv, head_dim=hd, out_dtype=torch.float32)
+    assert torch.equal(few[0], got[0][:200]) and torch.equal(few[1], got[1][:200])
 
 
 def test_one_key_stands_out(ops, gpu_device):
@@ -389,7 +444,7 @@ def test_idle_lanes_of_a_captured_step(ops, gpu_device):
 def test_graphs_replayed_beside_each_other(ops, gpu_device):
     """Two captured steps on two streams, each with shares to merge, and eager calls between."""
     nq, nkv, hd, made = 4, 2, 64, []
-    for i, spans in enumerate(([(900, 1), (5, 1)], [(300, 1), (1200, 1)])):
+    for i, spans in enumerate(([(4900, 1), (5, 1)], [(300, 1), (3200, 1)])):
         batch, whole, table, cache = scene(gpu_device, nkv=nkv, hd=hd, page=16, spans=spans, seed=i)
         k, v = heads_of(whole, nkv, hd, torch.bfloat16, gpu_device, 3 + i)
         ops.kv_store(k, v, whole, table, cache)

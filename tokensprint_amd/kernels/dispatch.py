@@ -151,16 +151,29 @@ class Dispatch:
     cooperative_workgroups: int = 512
     per_wave_workgroups: int = 4096
 
-    # ---- attention over keys and values of 4 bits: portions of at least `packed_portion` tokens have
-    # the kernel that makes tiles in LDS; of tiles of 16 rows (times key/value heads), up to
-    # `packed_items` have all their keys shared out evenly over workgroups (as many as the card holds at
-    # a time; `packed_workgroups` another number), more a wavefront each; up to so many chunks of 128
-    # keys an item is one workgroup's.
+    # ---- attention over keys and values of 4 bits.  An item is 16 query rows (tokens x query heads of a
+    # key/value head) and one key/value head; us with 8 key/value heads of 128, pages of 16.
+    #: steps of up to this many items are one launch, portions of prompts among them; above it
+    #: portions have the kernel that makes tiles in LDS for 128 rows (a prompt of 500 tokens of 16
+    #: heads, 504 items: 16 / 18; of 32 heads, 1,000 items: 29 / 18; 500 tokens behind 2,000: 43 / 54 and
+    #: 82 / 55; 30 single tokens beside 200 behind 2,000 of 16 heads: 37 / 68)
+    packed_few: int = 512
+    #: tokens from which a portion counts as one there (8 portions of 16 tokens behind 500 are
+    #: 10 as items and 19 in tiles, but 512 items of portions of 64 tokens and more 20 and 20, 1,024 36 and 21)
     packed_portion: int = 16
-    packed_items: int = 2048
-    packed_workgroups: int = 0
+    #: up to this many items a workgroup each (or their keys shared out, see the next), above it a
+    #: wavefront each (single tokens: 128 requests of 100 to 3,000 tokens, 1,024 items, 68 / 92; of 500, 32 /
+    #: 22; 160 requests of 100 to 3,000 98 / 114, of 500 39 / 31, 256 of 4,000 260 / 223; prompts of 4,000 tokens in
+    #: float32, 4,000 items, 361 / 243)
+    packed_items: int = 1024
+    #: contexts of up to this many tokens are a workgroup per item without a look at the lengths; longer
+    #: ones are shared out where the lengths on the device say so (1 request of 1,000: 9.7 whole, 11.5 with the
+    #: look; of 2,000 15 / 11; of 8,000 46 / 14; 4 requests of 1,300 12 / 14, of 2,500 18 / 13)
     packed_whole: int = 1280
+    #: the same for 1,024 items, which take turns (128 requests of 4,000: 121 / 130; of 1,300 52 / 59)
     packed_whole_many: int = 4096
+    #: workgroups that keys are shared out over; 0: one for each compute unit
+    packed_workgroups: int = 0
 
     # ---- recurrences.  A step whose longest portion has more tokens than this runs in chunks of
     # 64 tokens as products of matrices, below it every entry is walked whole by one launch.

@@ -1247,14 +1247,15 @@ class HipOps:
                 dtype is torch.bfloat16 and self.lib.ts_packed_prompt_fits(a.hd) == 1,
                 d.packed_workgroups or self.lib.ts_packed_resident())
         tall, resident = found
-        for portions in (True, False):
-            count, tiles = self._packed_tiles(batch, portions, 8 * tokens if portions and tall else tokens,
-                                              d.packed_portion)
+        if tall:         # few tiles of 16 rows have the one launch, portions of prompts too
+            tall = heads * self._packed_tiles(batch, None, tokens, 0)[0] > d.packed_few
+        for portions in (True, False) if tall else (None,):
+            count, tiles = self._packed_tiles(batch, portions, 8 * tokens if portions else tokens, d.packed_portion)
             if count == 0:
                 continue
             m.num_tiles, m.tiles = count, tiles
             items = count * heads
-            if portions and tall:
+            if portions:
                 # two sets of wavefronts share an item's keys where items leave units empty
                 self._call(self.lib.ts_packed_prompt, byref(m), 2 if items <= self._units else 1, c_void_p(stream))
                 continue
@@ -1262,7 +1263,7 @@ class HipOps:
             if shared:
                 reach = self._reach(a)
                 keys = batch.max_ctx_len if reach == 0 else min(batch.max_ctx_len, reach + batch.max_q_len + 64)
-                if keys > (d.packed_whole if items < 4 * self._units else d.packed_whole_many):
+                if keys > (d.packed_whole if items < d.packed_items else d.packed_whole_many):
                     workgroups = m.workgroups = resident
                     hd = -(-a.hd // 32) * 32
                     partial = torch.empty(workgroups * 32 * (hd + 2), dtype=torch.float32, device=self.device)
@@ -1273,15 +1274,15 @@ class HipOps:
 
     def _packed_tiles(self, batch, portions, tokens, least):
         """(number, device address or None) of the runs of at most `tokens` consecutive tokens of the
-        batch's entries that bring at least `least` tokens (`portions`), or of the others; those that see
-        most keys first.  A step of single tokens needs no list."""
+        batch's entries that bring at least `least` tokens (`portions`), of the others (False) or of all
+        (None); those that see most keys first.  A step of single tokens needs no list."""
         if batch.max_q_len == 1 and batch.num_tokens == batch.num_entries:
             return (0, None) if portions else (batch.num_entries, None)
         key = ("packed_tiles", portions, tokens, least)
         if key not in batch.plans:
             tiles, first = [], 0
             for entry, (n, start) in enumerate(zip(batch.q_lens, batch.starts)):
-                if (n >= least) == portions:
+                if portions is None or (n >= least) == portions:
                     tiles += [(start + min(t0 + tokens, n), entry, first + t0, min(tokens, n - t0))
                               for t0 in range(0, n, tokens)]
                 first += n
