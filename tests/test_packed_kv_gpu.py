@@ -441,6 +441,27 @@ def test_idle_lanes_of_a_captured_step(ops, gpu_device):
     assert torch.equal(cache.k_pages, before[0]) and torch.equal(cache.v_pages, before[1])
 
 
+def test_counts_made_in_inference_mode_are_reset_outside(gpu_device):
+    from tokensprint_amd.kernels.hip_ops import HipOps
+    ops = HipOps(gpu_device)
+    batch, whole, table, cache = scene(gpu_device, nkv=2, hd=64, page=16, spans=[(4000, 1), (7, 1)])
+    k, v = heads_of(whole, 2, 64, torch.bfloat16, gpu_device, 6)
+    q = rand((2, 4, 64), torch.bfloat16, gpu_device, 7)
+
+    def call():
+        return ops.paged_attention(q, batch, table, cache, num_heads=4, num_kv_heads=2, head_dim=64, scale=0.125,
+                                   window=None)
+
+    with torch.inference_mode():
+        ops.kv_store(k, v, whole, table, cache)
+        first = call()
+    ops.reset_scratch()
+    second = call()
+    with torch.inference_mode():
+        ops.reset_scratch()
+        assert torch.equal(call(), second) and torch.equal(first, second)
+
+
 def test_graphs_replayed_beside_each_other(ops, gpu_device):
     """Two captured steps on two streams, each with shares to merge, and eager calls between."""
     nq, nkv, hd, made = 4, 2, 64, []

@@ -222,7 +222,8 @@ class HipOps:
             if key[1]:               # what earlier captures used belongs to their graphs alone
                 for other in [k for k in self._count_arrays if k[1] not in (0, key[1])]:
                     del self._count_arrays[other]
-            counts = torch.zeros(max(n, 4096), dtype=torch.int32, device=self.device)
+            with torch.inference_mode(False):        # `reset_scratch` may come outside of it
+                counts = torch.zeros(max(n, 4096), dtype=torch.int32, device=self.device)
             self._count_arrays[key] = counts
         return counts
 
