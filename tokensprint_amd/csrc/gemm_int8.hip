@@ -231,9 +231,9 @@ extern "C" int ts_norm_quantize_rows(const float* resid, const void* delta, int 
 extern "C" int ts_linear_int8(const void* x, int x_type, const void* delta, int delta_type, const float* norm_w, float eps,
                               float* resid_out, void* rows, const void* w, const float* w_scale, void* c, int c_type,
                               int M, int N, int K, int row, int pair, float limit, hipStream_t stream) {
-  if (M <= 0 || N <= 0) return 0;
+  if (M <= 0) return 0;
   const uintptr_t used = (uintptr_t)x | (uintptr_t)delta | (uintptr_t)norm_w | (uintptr_t)resid_out | (uintptr_t)w | (uintptr_t)c;
-  if (M == 1 && (pair ? 2ll * N : N) <= 24576 && K >= 8 && K % 8 == 0 && row >= K && row % 256 == 0 && row <= kRowLongest &&
+  if (M == 1 && N > 0 && (pair ? 2ll * N : N) <= 24576 && K >= 8 && K % 8 == 0 && row >= K && row % 256 == 0 && row <= kRowLongest &&
       used % 16 == 0 && (c_type == TS_F32 || c_type == TS_BF16)) {
     const RowInt8Args a{{nullptr, (const signed char*)w, nullptr, w_scale, c, M, N, row, limit}, x, delta, norm_w, resid_out, K, eps};
 #define TS_ROW(T, TD, NORM, TC, PAIR) \
