@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import drives
-from helpers import FUBE, LAYER_E, PALE, PINE, SISE, TINY, ZOLO, random_prompt
+from helpers import FUBE, LAYER_E, PALE, PINE, SISE, TINY, ZOLO, ZONO, random_prompt
 from kernel_refs import TorchOps
 from packed_refs import quantize4
 from tokensprint_amd.engine import ModelRunner
@@ -52,7 +52,7 @@ class LowBitOps(TorchOps):
 
 
 MODELS = {"qwen3": TINY["B"], "qwen3 windowed": TINY["C"], "palelix": PALE["B"], "zolorax": ZOLO["B"],
-          "pinedra": PINE["B"], "fubepel": FUBE["B"], "sisepel": SISE["B"]}
+          "zonopel": ZONO["B"], "pinedra": PINE["B"], "fubepel": FUBE["B"], "sisepel": SISE["B"]}
 
 
 @pytest.fixture(scope="module", params=list(MODELS))
