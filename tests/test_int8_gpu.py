@@ -275,3 +275,43 @@ def test_one_call_with_a_row_that_is_not_finite(ops, value):
     got = ops.linear(x, weight, torch.float32)
     assert torch.equal(got[[0, 2]], want[[0, 2]])
     assert not torch.isfinite(got[1]).any()
+
+
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("rows,n,k", [(17, 4096, 4096), (64, 1000, 2048), (33, 2048, 8192), (128, 515, 12288),
+                                      (70, 96, 131072), (64, 4096, 5000)])
+def test_products_split_along_the_rows(ops, rows, n, k, pair):
+    """In parts that meet in memory, twice in a row, the bits are those of a tile that walks all of K; and so in
+    a graph's replays beside eager calls."""
+    torch.manual_seed(rows)
+    weight = ops.quantize_weight(torch.randn(n * (2 if pair else 1), k, device="cuda"))
+    x = ops.quantize_rows(torch.randn(rows, k, device="cuda"))
+    want = ops._int8_product(x, weight, torch.float32, pair=pair, tile=8)
+
+    def call():
+        return ops._int8_product(x, weight, torch.float32, pair=pair)
+
+    assert torch.equal(call(), want) and torch.equal(call(), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(call(), want) and torch.equal(out, want)
+
+
+def test_split_products_on_two_streams(ops):
+    made = []
+    for i in range(2):
+        weight = ops.quantize_weight(torch.randn(4096, 8192, device="cuda"))
+        x = ops.quantize_rows(torch.randn(40, 8192, device="cuda"))
+        made.append((x, weight, ops._int8_product(x, weight, torch.float32, tile=8), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for x, weight, want, stream in made:
+            with torch.cuda.stream(stream):
+                got.append((ops.linear(x, weight, torch.float32), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in got)

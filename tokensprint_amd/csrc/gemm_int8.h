@@ -19,6 +19,13 @@ struct Int8Args {
   float limit;               // pair: gated_unit's
 };
 
-// The kernel for many rows (gemm_int8_tiled.hip); whether it takes these sizes.
+// The kernel for many rows (gemm_int8_tiled.hip); whether it takes these sizes; into how many parts it would rather have K
+// split, and what memory that takes (bytes of partial sums, tiles).
+struct Int8Split {
+  int splits, tile, tiles;
+  int64_t bytes;
+};
+constexpr int kSplitRows = 128;
 bool gemm_int8_tiled_fits(int M, int N, int row, bool pair);
-int gemm_int8_tiled(const Int8Args& a, int c_type, bool pair, int tile, hipStream_t stream);
+Int8Split gemm_int8_split(int M, int N, int row, bool pair);
+int gemm_int8_tiled(const Int8Args& a, int c_type, bool pair, int tile, int* partial, unsigned* arrivals, hipStream_t stream);

@@ -195,17 +195,20 @@ static int launch_int8(const Int8Args& a, hipStream_t stream) {
 
 // Tiles from 5 rows on where the kernel above would be more than two workgroups a unit, of which every one reads its
 // rows of A for 16 rows of W alone (W [24576, 4096]: 1 row 24 us here, 26 in tiles; 16 rows 30 and 27.  [12288, 4096]:
-// 8 rows 15 and 15, 16 rows 17 and 15.  [4096, 4096]: 16 rows 8 and 10, 32 rows 10.5 and 10.5, 64 rows 18 and 11.
-// [1024, 4096]: 64 rows 6.0 and 7.5, 256 rows 16 and 7.4).
-static bool takes_few(int M, int N, bool pair) {
+// 8 rows 15 and 15, 16 rows 17 and 15.  [4096, 4096]: 16 rows 8 and 10), or from 17 rows more than one (tiles split
+// along K: [4096, 4096] 32 rows 10.5 and 8.8; [4096, 12288] 26.6 and 17.0; [1024, 4096] 64 rows 6.0 and 6.7), or
+// where rows are very long ([5120, 25600], 16 rows 56 and 35).
+static bool takes_few(int M, int N, int row, bool pair) {
   const int64_t workgroups = ((pair ? 2ll * N : N) + 15) / 16 * ((M + 15) / 16);
-  return M <= 4 || workgroups <= 512;
+  return M <= 4 || (row <= 16384 && workgroups <= (M <= 16 ? 512 : 256));
 }
 
 // `tile`: 0 lets the sizes choose the kernel; 1 to 8 name a tile of the kernel for many rows, 9 the one for few (for
-// measuring; the result is the same to the bit).
+// measuring; the result is the same to the bit).  `partial`: as much memory as ts_gemm_int8_split says, `arrivals` as many zeros;
+// null: K is not split.
 extern "C" int ts_gemm_int8(const void* x, const float* a_scale, const void* w, const float* w_scale, void* c,
-                            int c_type, int M, int N, int row, int pair, float limit, int tile, hipStream_t stream) {
+                            int c_type, int M, int N, int row, int pair, float limit, int tile, void* partial,
+                            unsigned* arrivals, hipStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   if (row <= 0 || row % 256 || row > 131072) TS_FAIL("gemm_int8: rows of %d bytes", row);
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)c) & 15) TS_FAIL("gemm_int8: operands must be 16-byte aligned");
@@ -214,8 +217,8 @@ extern "C" int ts_gemm_int8(const void* x, const float* a_scale, const void* w, 
   const Int8Args a{(const signed char*)x, (const signed char*)w, a_scale, w_scale, c, M, N, row, limit};
   const bool many = gemm_int8_tiled_fits(M, N, row, pair != 0);
   if (tile > 0 && tile < 9 && !many) TS_FAIL("gemm_int8: M=%d N=%d rows of %d bytes not taken in tiles", M, N, row);
-  const bool few = takes_few(M, N, pair != 0);
-  if (tile == 0 ? many && !few : tile < 9) return gemm_int8_tiled(a, c_type, pair != 0, tile, stream);
+  const bool few = takes_few(M, N, row, pair != 0);
+  if (tile == 0 ? many && !few : tile < 9) return gemm_int8_tiled(a, c_type, pair != 0, tile, (int*)partial, arrivals, stream);
   if (pair) return c_type == TS_BF16 ? launch_int8<bf16_t, true>(a, stream) : launch_int8<float, true>(a, stream);
   return c_type == TS_BF16 ? launch_int8<bf16_t, false>(a, stream) : launch_int8<float, false>(a, stream);
 }
@@ -226,11 +229,21 @@ extern "C" int ts_norm_quantize_rows(const float* resid, const void* delta, int 
                                      float* resid_out, void* codes, float* scales, int M, int K, int row,
                                      hipStream_t stream);
 
+// Bytes of partial sums with which a product of these sizes is split along K, or 0, and the tiles that count themselves in.
+extern "C" int64_t ts_gemm_int8_split(int M, int N, int row, int pair, int* tiles) {
+  *tiles = 0;
+  if (M <= 0 || N <= 0 || row <= 0 || takes_few(M, N, row, pair != 0)) return 0;
+  const Int8Split s = gemm_int8_split(M, N, row, pair != 0);
+  *tiles = s.tiles;
+  return s.bytes;
+}
+
 // Rows into 8 bits and their product.  `norm_w` null: x as it is; else x is the float32 stream, `delta` (or null) is
 // added to it, the sum goes into `resid_out` and the rows are normed.  `rows`: M (row + 4) bytes of scratch memory.
 extern "C" int ts_linear_int8(const void* x, int x_type, const void* delta, int delta_type, const float* norm_w, float eps,
                               float* resid_out, void* rows, const void* w, const float* w_scale, void* c, int c_type,
-                              int M, int N, int K, int row, int pair, float limit, hipStream_t stream) {
+                              int M, int N, int K, int row, int pair, float limit, void* partial, unsigned* arrivals,
+                              hipStream_t stream) {
   if (M <= 0) return 0;
   const uintptr_t used = (uintptr_t)x | (uintptr_t)delta | (uintptr_t)norm_w | (uintptr_t)resid_out | (uintptr_t)w | (uintptr_t)c;
   if (M == 1 && N > 0 && (pair ? 2ll * N : N) <= 24576 && K >= 8 && K % 8 == 0 && row >= K && row % 256 == 0 && row <= kRowLongest &&
@@ -252,5 +265,5 @@ extern "C" int ts_linear_int8(const void* x, int x_type, const void* delta, int 
   const int rc = norm_w ? ts_norm_quantize_rows((const float*)x, delta, delta_type, norm_w, eps, resid_out, rows, scales, M,
                                                 K, row, stream)
                         : ts_quantize_rows(x, x_type, rows, scales, M, K, row, stream);
-  return rc ? rc : ts_gemm_int8(rows, scales, w, w_scale, c, c_type, M, N, row, pair, limit, 0, stream);
+  return rc ? rc : ts_gemm_int8(rows, scales, w, w_scale, c, c_type, M, N, row, pair, limit, 0, partial, arrivals, stream);
 }

@@ -74,6 +74,11 @@ struct TiledHeadsArgs : TiledArgs {
 
 struct TiledInt8Args : TiledArgs {
   const float *a_scale, *w_scale;     // [M], [N] (PAIR: [2 N])
+  // K in `splits` parts, a workgroup each: their whole sums meet in `partial` [tiles, splits, a tile's sums], the last of
+  // a tile's to come (`arrivals` [tiles], left as zeros) adds them up
+  int splits;
+  int* partial;
+  unsigned* arrivals;
 };
 
 constexpr int kPlain = 0, kScaled = 1, kTail = 2, kHeads = 3, kInt8 = 4;
@@ -253,6 +258,12 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
   const int height = min(g.panel, g.tiles_m - panel * g.panel);
   const int tile_m = panel * g.panel + in_panel % height, tile_n = in_panel / height;
   const int m0 = tile_m * BM;
+  int KT = g.K / 64;                                 // K steps, at least STAGES (the launcher's check)
+  if constexpr (FORM == kInt8) {
+    const int each = (KT + g.splits - 1) / g.splits, first = (int)blockIdx.y * each;
+    g.a += (int64_t)first * 64, g.w += (int64_t)first * 64;
+    KT = min(each, KT - first);
+  }
 
   // SCALED: the factors of this tile's rows.  Called once the first direct loads are on
   // their way and before the K loop counts loads: these loads are waited for with all
@@ -413,7 +424,6 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
   // kt + 1 has arrived and step kt has been read by everyone) its second half while the
   // first half of step kt + 1 comes out of LDS and the loads of step kt + STAGES go out
   // into the buffer that step kt has left.
-  const int KT = g.K / 64;                              // at least STAGES (the launcher's check)
   if constexpr (TM * TN > 16) {
     // A wave's part is too large to hold two K steps' operands beside its sums.  A turn (one K
     // step) is walked in blocks of TN products, a row block of A against the wave's columns:
@@ -642,6 +652,32 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
     return;
   }
   if constexpr (FORM == kInt8) {
+    if (g.splits > 1) {
+      // (stores and loads that pass the L2, which the other parts' units may not share)
+      __shared__ unsigned before;
+      constexpr int SUMS = TN * TM * 4, THREADS = 64 * NW;
+      int* mine = g.partial + ((int64_t)tile * g.splits + blockIdx.y) * SUMS * THREADS + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < SUMS; ++i)
+        __hip_atomic_store(mine + i * THREADS, acc[i / 4 / TM][i / 4 % TM][i % 4], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      if (threadIdx.x == 0) before = __hip_atomic_fetch_add(g.arrivals + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if ((int)before + 1 != g.splits) return;
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+      if (threadIdx.x == 0) __hip_atomic_store(g.arrivals + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int s = 0; s < g.splits; ++s) {
+        if (s == (int)blockIdx.y) continue;
+        const int* other = g.partial + ((int64_t)tile * g.splits + s) * SUMS * THREADS + threadIdx.x;
+        int v[SUMS];
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) v[i] = __hip_atomic_load(other + i * THREADS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) acc[i / 4 / TM][i / 4 % TM][i % 4] += v[i];
+      }
+    }
     constexpr int COLS = PAIR ? TN / 2 : TN;
     auto scales = [&](const float* p, int n) {
       f32x4 s;
@@ -741,7 +777,13 @@ int launch_tiled(TiledArgsOf<FORM> g, hipStream_t stream) {
     const int64_t rows = (int64_t)(p < g.tiles_m ? p : g.tiles_m) * BM + (int64_t)((held + p - 1) / p) * BN;
     if (best_rows < 0 || rows < best_rows) { best_rows = rows; g.panel = p; }
   }
-  hipLaunchKernelGGL(kernel, dim3(8 * per_xcd), dim3(64 * GM * GN), lds, stream, g);
+  unsigned parts = 1;
+  if constexpr (FORM == kInt8) {
+    parts = (unsigned)g.splits;
+    const int steps = g.K / 64, each = (steps + g.splits - 1) / g.splits;
+    if (steps - each * (g.splits - 1) < STAGES) TS_FAIL("gemm_tiled: K=%d is too short for %d parts", g.K, g.splits);
+  }
+  hipLaunchKernelGGL(kernel, dim3(8 * per_xcd, parts), dim3(64 * GM * GN), lds, stream, g);
   TS_CHECK_LAUNCH("gemm_tiled");
   return 0;
 }

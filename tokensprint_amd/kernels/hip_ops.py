@@ -103,8 +103,8 @@ _ARGUMENTS = {
     "ts_pack_values": "ppppi" + "ppp" + "iiiii" + "p",
     "ts_quantize_rows": "pi" + "pp" + "iii" + "p",
     "ts_norm_quantize_rows": "ppipf" + "ppp" + "iii" + "p",
-    "ts_gemm_int8": "ppppp" + "iiiii" + "f" + "i" + "p",
-    "ts_linear_int8": "pi" + "pipfp" + "pppp" + "iiiii" + "if" + "p",
+    "ts_gemm_int8": "ppppp" + "iiiii" + "f" + "i" + "pp" + "p",
+    "ts_linear_int8": "pi" + "pipfp" + "pppp" + "iiiii" + "if" + "pp" + "p",
 }
 
 
@@ -116,6 +116,7 @@ def _load_library() -> ctypes.CDLL:
     lib.ts_last_error.restype = ctypes.c_char_p
     lib.ts_chunked_scratch.restype = c_int64
     lib.ts_capture_id.restype = c_int64
+    lib.ts_gemm_int8_split.restype = c_int64
     # (with their types named, addresses go in as the numbers that they are, not each in an object of its own)
     for name, args in _ARGUMENTS.items():
         getattr(lib, name).argtypes = [_LETTERS[c] for c in args]
@@ -996,10 +997,28 @@ class HipOps:
         self._check("x codes", x.codes, torch.int8, shape=(M, row))
         self._check("x scales", x.scales, torch.float32, shape=(M,))
         out = torch.empty(M, N, dtype=out_dtype, device=self.device)
+        partial, counts = self._int8_split(M, N, row, pair)
         self._call(self.lib.ts_gemm_int8, x.codes.data_ptr(), x.scales.data_ptr(), weight.codes.data_ptr(),
                    weight.scales.data_ptr(), out.data_ptr(), _TYPE_CODE[out_dtype], M, N, row, int(pair),
-                   unit or 0.0, tile, self._raw_stream(self._device_index))
+                   unit or 0.0, tile, None if partial is None else partial.data_ptr(), counts,
+                   self._raw_stream(self._device_index))
         return out
+
+    def _int8_split(self, M, N, row, pair):
+        """Memory for a product whose K is split over workgroups (few rows, a narrow weight), and the zeros in
+        which they count themselves in."""
+        if M > 128:              # (the library says 0 from there on)
+            return None, None
+        key = "int8", M, N, row, pair
+        found = self._routes.get(key) if self._routes_of is self.dispatch else None
+        if found is None:
+            tiles = c_int(0)
+            found = self._kept_routes()[key] = (
+                self.lib.ts_gemm_int8_split(M, N, row, int(pair), byref(tiles)), tiles.value)
+        size, tiles = found
+        if size == 0:
+            return None, None
+        return torch.empty(size, dtype=torch.int8, device=self.device), self._counts(tiles).data_ptr()
 
     def _int8_linear(self, x, delta, norm_weight, eps, stream_out, weight, out_dtype, pair, unit):
         """Rows (with a norm weight: of the stream, added to and normed) into 8 bits and their product, in
@@ -1008,13 +1027,15 @@ class HipOps:
         N, row = self._int8_weight(weight, K, out_dtype, pair)
         out = torch.empty(M, N, dtype=out_dtype, device=self.device)
         rows = torch.empty(M * (row + 4), dtype=torch.int8, device=self.device)      # numbers, then scales
+        partial, counts = self._int8_split(M, N, row, pair)
         added = delta is not None
         self._call(self.lib.ts_linear_int8, x.data_ptr(), _TYPE_CODE[x.dtype],
                    delta.data_ptr() if added else None, _TYPE_CODE[delta.dtype] if added else 0,
                    None if norm_weight is None else norm_weight.data_ptr(), eps,
                    stream_out.data_ptr() if added else None, rows.data_ptr(), weight.codes.data_ptr(),
                    weight.scales.data_ptr(), out.data_ptr(), _TYPE_CODE[out_dtype], M, N, K, row,
-                   int(pair), unit or 0.0, self._raw_stream(self._device_index))
+                   int(pair), unit or 0.0, None if partial is None else partial.data_ptr(), counts,
+                   self._raw_stream(self._device_index))
         return out
 
     # ------------------------------------------------------------ q/k preparation
