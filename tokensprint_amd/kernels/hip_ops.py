@@ -1270,7 +1270,10 @@ class HipOps:
                 d.packed_workgroups or self.lib.ts_packed_resident())
         tall, resident = found
         if tall:         # few tiles of 16 rows have the one launch, portions of prompts too
-            tall = heads * self._packed_tiles(batch, None, tokens, 0)[0] > d.packed_few
+            key = "packed_count", tokens
+            if key not in batch.plans:
+                batch.plans[key] = sum(-(-n // tokens) for n in batch.q_lens)
+            tall = heads * batch.plans[key] > d.packed_few
         for portions in (True, False) if tall else (None,):
             count, tiles = self._packed_tiles(batch, portions, 8 * tokens if portions else tokens, d.packed_portion)
             if count == 0:
