@@ -467,7 +467,7 @@ __device__ __forceinline__ void packed_plan(const PackedArgs& args, int heads, i
 // that an earlier one began, the part that a later one goes on with), and whoever comes last merges them in their order, sixteen
 // parts asked for at a time (four: 25 us in place of 18 for that request).
 //
-// Not SHARED: an item a workgroup, without that look (1 us).
+// Not SHARED: an item a workgroup, without that look (2 us).
 template <int NB, bool WIDE>
 struct PackedShape {
   static constexpr int WAVES = 4 * packed_waves(NB, WIDE), THREADS = WAVES * kWave;
