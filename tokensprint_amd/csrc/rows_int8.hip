@@ -129,7 +129,7 @@ static int launch_quant_rows(const QuantRowsArgs& a, hipStream_t stream) {
   // of 5,120: 28 us, 4.5 TB/s; with 640 threads 38; with 64 31).
   const int most = NORM || a.M <= 512 ? 1024 : pieces <= 1536 ? 256 : 512;
   const int each = (pieces + most - 1) / most, threads = ((pieces + each - 1) / each + 63) / 64 * 64;
-  if (a.K % 8 || (used & 15) || pieces > 4096) TS_ROWS(0, 512);
+  if (a.K % 8 || (used & 15) || pieces > 4096) TS_ROWS(0, a.K < 512 ? (a.K + 63) / 64 * 64 : 512);
   else if (each == 1) TS_ROWS(1, threads);
   else if (each == 2) TS_ROWS(2, threads);
   else if constexpr (NORM) TS_ROWS(4, threads);
