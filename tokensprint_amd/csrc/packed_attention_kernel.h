@@ -10,6 +10,11 @@
 // Sums of q over a group are float32 numbers of a query row, that is of a lane, and start the group's product as
 // -(16 + zero) sum(q); p step is rounded to float16 once and meets codes and -(16 + zero) (a product with the same numbers in
 // every row) alike, so what its rounding costs is in proportion to the value.
+// Float16 holds 11 bits from 2^-14 on only, and a key far below the row's largest score, or values far below 1, would
+// lose them (of 4,000 keys 12 below one that has no value itself, with values of 0.02, a tenth of the result, while the
+// row's sum of weights keeps them).  So steps are brought up first, by the power of two that puts the largest of the
+// wavefront's keys so far below 2^15 (PackedLift): p step has all its bits from 2^-28 of that on, a
+// weight of 4e-9 where steps are alike.  Three instructions more for 32 keys than without.
 // A wavefront dequantises nothing: seven instructions make a word of eight codes operands, a score costs two
 // multiplications a group and a weight one.
 //
@@ -153,14 +158,37 @@ __device__ __forceinline__ u32x4 packed_scale_of(unsigned word, int i) {      //
   return packed_scale<3>(word);
 }
 
+// By how much a wavefront's steps are brought up: the power of two that takes the largest so far from below
+// 2^(exponent - 14) to below 2^15, in two factors that float16 holds (a lane of biases: 1).  Steps are float16 numbers, so
+// this is exact, and with it all that follows from it but the bits that small weights would lose.
+struct PackedLift {
+  int exponent;            // float16's field of the largest step so far (0 below 2^-14); the same in all lanes
+  f16x2 by[2];             // of this lane's word
+  __device__ __forceinline__ static PackedLift none(int lane) { return at(0, lane); }
+  __device__ __forceinline__ static PackedLift at(int exponent, int lane) {
+    // 2^(29 - exponent), -1 to 29, as 2^half and 2^(the rest)
+    const int up = 29 - exponent, half = up >> 1;
+    const bool bias = lane % 4 >= 2;
+    const _Float16 one = (_Float16)1.f;
+    const _Float16 a = bias ? one : (_Float16)ldexpf(1.f, half), b = bias ? one : (_Float16)ldexpf(1.f, up - half);
+    return PackedLift{exponent, {f16x2{a, a}, f16x2{b, b}}};
+  }
+  __device__ __forceinline__ float down() const { return ldexpf(1.f, exponent - 29); }
+  __device__ __forceinline__ unsigned raised(unsigned word) const {
+    return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, word) * by[0] * by[1]);
+  }
+};
+
 template <int NB, bool WIDE>
 struct PackedTile {
   static constexpr int NG = (NB + 1) / 2;        // groups that exist
   u32x4 q[WIDE ? 2 : 1][NB]; // bfloat16, or two parts in float16
   float qsum[NG];            // the row's sum over each group; WIDE: qsum[0] is what turns a product into q . k
   f32x4 o[2 * NB], oz[WIDE ? 2 * NB : NG];       // oz: the zeros' share; WIDE: sums of the second parts
+  PackedLift lift;           // o and oz count so many times
   float m, l;
   int pos, lo, keep;
+  int last, first;           // of all rows: the last key, and the first one that is not behind the window
 };
 
 // The parts of eight numbers: 11 bits, and 2^up times the next 11.
@@ -221,6 +249,7 @@ __device__ __forceinline__ void load_packed_query(PackedTile<NB, WIDE>& t, const
   for (int i = 0; i < (WIDE ? 2 * NB : NG); ++i) t.oz[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int db = 0; db < 2 * NB; ++db) t.o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  t.lift = PackedLift::none(threadIdx.x % kWave);
   t.m = -INFINITY;
   t.l = 0.f;
 }
@@ -274,8 +303,17 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, WIDE>& t, const Pac
       for (int j = 0; j < 4; ++j) st[blk][j] = extra_score_log2(*x, st[blk][j], kb + blk * 16 + g * 4 + j);
     scale_log2 = 1.f;
   }
+  unsigned steps[2] = {b.vs[0], b.vs[1]};        // with their biases
   if (!interior || (b.page[0] | b.page[1]) < 0) {
     asm volatile("" ::: "memory");       // keeps this a branch
+    // (steps that a page holds of nobody's keys are none: they have no say in the lift)
+    const int word = threadIdx.x % 4;
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      const int key = kb + blk * 16 + g * 4 + word * 2;
+      auto there = [&](int k) { return b.page[blk] >= 0 && k <= t.last && (k >= t.first || k < t.keep); };
+      if (word < 2) steps[blk] &= (there(key) ? 0xffffu : 0u) | (there(key + 1) ? 0xffff0000u : 0u);
+    }
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
@@ -296,20 +334,34 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, WIDE>& t, const Pac
   }
   t.l = t.l * corr + sum;
   t.m = m_new;
+  // the block's largest step (as whole numbers float16's order is theirs, and biases are below all)
+  typedef __attribute__((ext_vector_type(2))) short i16x2;
+  const i16x2 top2 = __builtin_elementwise_max(__builtin_bit_cast(i16x2, steps[0]), __builtin_bit_cast(i16x2, steps[1]));
+  const int top = max((int)top2[0], (int)top2[1]);
+  float change = corr;
+  if (__builtin_amdgcn_ballot_w64(top >= (t.lift.exponent + 1) << 10) != 0) {
+    int exponent = 0;
+#pragma unroll
+    for (int bit = 16; bit > 0; bit >>= 1)
+      if (__builtin_amdgcn_ballot_w64(top >= (exponent + bit) << 10) != 0) exponent += bit;
+    change *= ldexpf(1.f, t.lift.exponent - exponent);
+    t.lift = PackedLift::at(exponent, threadIdx.x % kWave);
+  }
   // (far into a context most blocks bring no new largest score)
-  if (__builtin_amdgcn_ballot_w64(corr != 1.f) != 0) {
+  if (__builtin_amdgcn_ballot_w64(change != 1.f) != 0) {
 #pragma unroll
     for (int db = 0; db < 2 * NB; ++db)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) t.o[db][j] *= corr;
+      for (int j = 0; j < 4; ++j) t.o[db][j] *= change;
 #pragma unroll
     for (int i = 0; i < (WIDE ? 2 * NB : NG); ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) t.oz[i][j] *= corr;
+      for (int j = 0; j < 4; ++j) t.oz[i][j] *= change;
   }
+  steps[0] = t.lift.raised(steps[0]), steps[1] = t.lift.raised(steps[1]);
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
-    const u32x4 s0 = packed_scale_of<PackedBlock<NB>::G>(b.vs[0], i), s1 = packed_scale_of<PackedBlock<NB>::G>(b.vs[1], i);
+    const u32x4 s0 = packed_scale_of<PackedBlock<NB>::G>(steps[0], i), s1 = packed_scale_of<PackedBlock<NB>::G>(steps[1], i);
     if constexpr (!WIDE) {
       // (a multiplication and its rounding to float16 are one instruction)
       f16x8 w;
@@ -346,13 +398,15 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, WIDE>& t, const Pac
   }
 }
 
-// The rows' sums with what the zeros take off, or with the second parts.
+// The rows' sums with what the zeros take off, or with the second parts, as often as they count.
 template <int NB, bool WIDE>
 __device__ __forceinline__ void packed_finish(PackedTile<NB, WIDE>& t) {
+  const float down = t.lift.down();
 #pragma unroll
   for (int db = 0; db < 2 * NB; ++db)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) t.o[db][j] = WIDE ? fmaf(t.oz[db][j], 1.f / 2048.f, t.o[db][j]) : t.o[db][j] + t.oz[db / 4][j];
+    for (int j = 0; j < 4; ++j)
+      t.o[db][j] = down * (WIDE ? fmaf(t.oz[db][j], 1.f / 2048.f, t.o[db][j]) : t.o[db][j] + t.oz[db / 4][j]);
   t.l = col4_sum(t.l);
 }
 
@@ -537,6 +591,7 @@ __global__ __launch_bounds__((PackedShape<NB, WIDE>::THREADS), packed_waves(NB, 
     t.pos = row_ok ? it.pos_first + ti : -1;
     t.lo = first_visible(a, t.pos);
     t.keep = a.keep;
+    t.last = it.pos_last, t.first = first_visible(a, it.pos_first);
     load_packed_query<NB, WIDE, T>(t, (const T*)a.q + ((int64_t)token * a.nq + head) * a.hd, row_ok, a.hd, g);
     ScoreExtraLog2 x;
     if (EXTRA) x = in_log2(score_extra(a, head, t.pos));
@@ -678,6 +733,7 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_walk_kerne
   t.pos = row_ok ? it.pos_first + ti : -1;
   t.lo = first_visible(a, t.pos);
   t.keep = a.keep;
+  t.last = it.pos_last, t.first = first_visible(a, it.pos_first);
   load_packed_query<NB, WIDE, T>(t, (const T*)a.q + ((int64_t)token * a.nq + head) * a.hd, row_ok, a.hd, g);
   ScoreExtraLog2 x;
   if (EXTRA) x = in_log2(score_extra(a, head, t.pos));

@@ -27,7 +27,8 @@
 // A code c becomes the bfloat16 number 16 + c by putting its bits behind the leading bit of 16, so a word
 // gives eight operands in seven instructions: (word >> 4 i) & 0x00780078 | 0x41804180; values the same in float16 (0x03c003c0,
 // 0x4c004c00), because a weight times a step is rounded to float16, an eighth of bfloat16's error, in the instruction that
-// multiplies (weights are at most 1 and steps float16 numbers: nothing overflows).  For that a
+// multiplies (steps are brought up to stand high in float16's range first, so neither does it overflow nor do small
+// weights lose bits: PackedLift in packed_attention_kernel.h).  For that a
 // word of keys is kept turned left by three bits, one of values by six.  Code p of a word (before turning: bits 4 p .. 4 p + 3) is
 // element j = 2 p of keys for p < 4, 2 (p - 4) + 1 else; of values, token i of the first element for p = i / 2 + 4
 // (i % 2), of the second 2 further.
