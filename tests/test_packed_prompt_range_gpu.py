@@ -1,0 +1,65 @@
+"""Prompts' attention over keys and values of 4 bits where its numbers are far apart."""
+
+import dataclasses
+
+import pytest
+import torch
+
+from test_packed_kv_gpu import rand, scene
+from test_packed_range_gpu import (BF16, F32, TOLERANCE, assert_pages_are_of_no_consequence, peaked, relative, run)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(gpu_device):
+    """All portions by the kernel that makes tiles in LDS."""
+    from tokensprint_amd.kernels import load_hip_ops
+    ops = load_hip_ops(gpu_device)
+    before = ops.dispatch
+    ops.dispatch = dataclasses.replace(before, packed_few=0, packed_portion=1)
+    yield ops
+    ops.dispatch = before
+
+
+# (as for single tokens, beside a float16 rounding of every key's and value's number: values' of 2^-11 at the most,
+# independent of the weights' and of each other)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("above,std,place", [(8, 0.02, 0), (12, 0.1, 0), (12, 0.02, 1777), (14, 0.02, 0), (14, 0.1, 3000),
+                                             (10, 1e-3, 0), (14, 1e-3, 900), (12, 5e-3, 0),
+                                             (16.875, 0.05, 0), (16.875, 5e-3, 1000), (14.0625, 0.02, 0)])
+def test_one_key_of_no_value_far_above_the_rest(ops, gpu_device, hd, above, std, place):
+    got, want = run(ops, *peaked(gpu_device, BF16, nq=4, nkv=2, hd=hd, spans=[(4000, 24), (1800, 17)], above=above, std=std,
+                                 place=place))
+    worst = relative(got, want)
+    assert worst <= TOLERANCE[BF16]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_more_items_than_units(ops, gpu_device, hd):
+    """Where items fill the card one set of wavefronts has all of an item's keys, else two share them."""
+    spans = [(1200 + 3 * i, 2) for i in range(130)]
+    assert 2 * len(spans) > ops._units
+    got, want = run(ops, *peaked(gpu_device, BF16, nq=4, nkv=2, hd=hd, spans=spans, above=14, std=0.05, place=7))
+    # The key's number is rounded to 11 bits: of a score of 14 (a step of 0.93310546875, a number of
+    # 15 / 16 of it, 0.87478638, which becomes 0.875) that is 13.9966 x 2.441e-4 = 3.417e-3, by which all the others'
+    # weights shrink together.
+    worst = relative(got, want)
+    assert worst <= TOLERANCE[BF16] + 3.43e-3
+
+
+def test_what_the_pages_held_before_is_of_no_consequence(ops, gpu_device):
+    args = peaked(gpu_device, BF16, nq=4, nkv=2, hd=64, spans=[(300, 23), (40, 30), (1505, 3)], above=14, std=1e-3, place=0)
+    assert_pages_are_of_no_consequence(ops, gpu_device, args, BF16)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_ordinary_numbers_to_the_types_rounding(ops, gpu_device, hd):
+    nq, nkv = 4, 2
+    batch, whole, table, cache = scene(gpu_device, nkv=nkv, hd=hd, page=16, spans=[(800, 30), (0, 20)])
+    k, v = rand((whole.num_tokens, nkv, hd), BF16, gpu_device, 1), rand((whole.num_tokens, nkv, hd), BF16, gpu_device, 2)
+    q = rand((batch.num_tokens, nq, hd), BF16, gpu_device, 3, 1.0 if hd == 64 else 0.7)
+    got, want = run(ops, q, k, v, batch, whole, table, cache, nkv)
+    # (a key's 11 bits too: hd independent roundings of 2^-11 |k q|, scores to 2^-9 of their deviation of 1)
+    worst = relative(got, want)
+    assert worst <= TOLERANCE[BF16] + 2.0 ** -9

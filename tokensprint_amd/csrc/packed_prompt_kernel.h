@@ -4,7 +4,10 @@
 // A turn is 64 keys, four blocks of a page; a wavefront turns one block's codes into float16 numbers step (code - zero) / 16
 // and writes them where its operands are read, 15 instructions for eight of them, once for the 128 rows of an item. The
 // sixteenth keeps every step in float16's range; queries are float16 as well, scaled by a power of two a row (their
-// bfloat16 bits are exact then), and so are weights. What is rounded is a key's or a value's number, to 11 bits.  (As
+// bfloat16 bits are exact then), and so are weights, which count 2^15 times: as they are, 9 below the row's largest score
+// they would have fewer than 11 bits, and 17 below none (4,000 keys 14 below one of no value: 0.6 % of the result; now
+// bits go from 20 below on).  What is rounded is a key's or a value's number, to 11 bits (a score s that one element
+// makes alone is off by 2^-11 s at the most).  (As
 // step (16 + code) less a rounded step (16 + zero), in 4 instructions less, results were three times as far off.)
 // The next turn's codes, asked for a turn ahead, become numbers between the scores' products, a word a step, and the second
 // half of a turn's weights are made between the first half's products: a turn is one meeting of the workgroup.
@@ -22,6 +25,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
   constexpr int SUB = HD / 32;                 // slots of 1 KB per sixteen keys
   constexpr int VALUES = KEYS * HD * 2;        // bytes of a turn's keys; its values lie behind them
   constexpr int BUF = 2 * VALUES;
+  constexpr float kUp = 15.f;                  // weights, their sums and o count 2^kUp times, values' numbers a sixteenth
   static_assert((HD == 64 || HD == 128) && G == TILES, "rows of 128 or 256 bytes, a block a wavefront");
   extern __shared__ __attribute__((aligned(1024))) unsigned char prefill_lds[];
   const AttentionArgs& a = args.base;
@@ -266,13 +270,13 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[db][i] *= corr;
     }
-    const float m_use = max2(m, -1e30f);
+    const float rise = kUp - max2(m, -1e30f);
     // the first block's weights, then its values' products between those of the second
     f16x8 pv[G];
     // (the row's sum is of the weights as they enter the products, two at a time)
     float before = 0.f;
     auto weight = [&](int b, int i) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][i], scale_log2, -m_use));
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][i], scale_log2, rise));
       if (i % 2 == 0) {
         before = p;
         return;
@@ -321,7 +325,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     meet();
   }
 
-  l = halves_sum(l);                           // (by all lanes: it crosses lanes)
+  l = halves_sum(l) * 0x1p-15f;                // (by all lanes: it crosses lanes)
   bf16_t* out = (bf16_t*)a.out + ((int64_t)(tok0 + ti) * a.nq + head) * HD;
   // Unit u of the results: registers 8 (u % 2) .. + 7 of o[u / 2], elements 16 u + 4 h .. + 3 and
   // 16 u + 8 + 4 h .. + 3.  The lane's halves exchange four each, and a lane has eight in a row.
@@ -339,7 +343,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
   };
   if constexpr (SETS == 1) {
     const float sum = sum_with_sink(l, m, a.sink, head);
-    const float inv = sum > 0.f ? 16.f / sum : 0.f;
+    const float inv = sum > 0.f ? 0x1p-11f / sum : 0.f;
 #pragma unroll
     for (int u = 0; u < 2 * DB; ++u) {
       float v[8];
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
       sum += lds_ml[((s * TILES + wave) * 2 + 1) * kWave + lane] * w[s];
     }
     sum = sum_with_sink(sum, m_use, a.sink, head);
-    const float inv = sum > 0.f ? 16.f / sum : 0.f;
+    const float inv = sum > 0.f ? 0x1p-11f / sum : 0.f;
 #pragma unroll
     for (int n = 0; n < UNITS; ++n) {
       const int u = set * UNITS + n;
