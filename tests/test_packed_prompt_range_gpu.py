@@ -63,3 +63,25 @@ def test_ordinary_numbers_to_the_types_rounding(ops, gpu_device, hd):
     # (a key's 11 bits too: hd independent roundings of 2^-11 |k q|, scores to 2^-9 of their deviation of 1)
     worst = relative(got, want)
     assert worst <= TOLERANCE[BF16] + 2.0 ** -9
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_steps_keep_their_bits(ops, gpu_device, hd):
+    """Steps of 2^-14 to 2^-13, held in 10 to 11 bits; codes of 0 and 15 alone, so that numbers are not small beside
+    float16's smallest ones where the steps are."""
+    nq, nkv = 4, 2
+    batch, whole, table, cache = scene(gpu_device, nkv=nkv, hd=hd, page=16, spans=[(600, 40), (0, 33)])
+    T = whole.num_tokens
+    size = (15 * 2.0 ** -14 * (1 + torch.rand(T, nkv, 1, generator=torch.Generator().manual_seed(1)))).to(gpu_device)
+    on = (rand((T, nkv, hd), F32, gpu_device, 2) > 0).float()
+    sign = rand((T, nkv, 1), F32, gpu_device, 3).sign()
+    v = (size * on * sign).to(BF16)
+    k = torch.zeros(T, nkv, hd, dtype=BF16, device=gpu_device)
+    k[:, :, 0] = (15 * 2.0 ** -13 * rand((T, nkv), F32, gpu_device, 4).clamp(-1, 1)).to(BF16)
+    q = torch.zeros(batch.num_tokens, nq, hd, dtype=BF16, device=gpu_device)
+    q[:, :, 0] = 4 * 4096.0
+    got, want = run(ops, q, k, v, batch, whole, table, cache, nkv)
+    # as TOLERANCE; numbers have 11 bits from 2^-14 on (a key's, of 15 steps / 16: scores of up to 3.8 to 2^-11
+    # at the most, 2e-3 of a weight, independent)
+    worst = relative(got, want)
+    assert worst <= 2.0 ** -8 + 2.0 ** -9

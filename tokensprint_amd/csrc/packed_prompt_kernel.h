@@ -3,11 +3,11 @@
 //
 // A turn is 64 keys, four blocks of a page; a wavefront turns one block's codes into float16 numbers step (code - zero) / 16
 // and writes them where its operands are read, 15 instructions for eight of them, once for the 128 rows of an item. The
-// sixteenth keeps every step in float16's range; queries are float16 as well, scaled by a power of two a row (their
+// sixteenth keeps every number in float16's range; queries are float16 as well, scaled by a power of two a row (their
 // bfloat16 bits are exact then), and so are weights, which count 2^15 times: as they are, 9 below the row's largest score
 // they would have fewer than 11 bits, and 17 below none (4,000 keys 14 below one of no value: 0.6 % of the result; now
 // bits go from 20 below on).  What is rounded is a key's or a value's number, to 11 bits (a score s that one element
-// makes alone is off by 2^-11 s at the most).  (As
+// makes alone is off by 2^-11 s at the most), and to 2^-21 where it is below 2^-10: a 32nd of a step of 2^-16.  (As
 // step (16 + code) less a rounded step (16 + zero), in 4 instructions less, results were three times as far off.)
 // The next turn's codes, asked for a turn ahead, become numbers between the scores' products, a word a step, and the second
 // half of a turn's weights are made between the first half's products: a turn is one meeting of the workgroup.
@@ -141,15 +141,16 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     }
     fetch_id(v + KEYS * SETS);
   };
-  // Codes into the tile, a word of a lane's at a time (keys, then values): 16 + c, less 16 + zero (exact), times a sixteenth of
-  // the step.
+  // Codes into the tile, a word of a lane's at a time (keys, then values): 1 + c / 16, less 1 + zero / 16 (exact), times the step.
+  // (The sixteenth on the step instead cost steps below 2^-10 their last bits, for every number of a group: at
+  // 2^-14 four of eleven, and results were 0.8 % off.)
   auto unpack = [&](unsigned char* buf, int n) {
     const _Float16 sixteenth = (_Float16)0.0625f;
     if (n < NB) {
       const int b = n;
       unsigned w[4];
-      whole_keys(kw[b], kz[b / 2], w);
-      const _Float16 s1 = __builtin_bit_cast(_Float16, (unsigned short)ks[b / 2]) * sixteenth;
+      whole_keys<true>(kw[b], __builtin_bit_cast(_Float16, (unsigned short)kz[b / 2]) * sixteenth, w);
+      const _Float16 s1 = __builtin_bit_cast(_Float16, (unsigned short)ks[b / 2]);
       const f16x2 s = {s1, s1};
       u32x4 out;
 #pragma unroll
@@ -160,10 +161,11 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     } else {
       const int b = n - NB;
       const u32x4 scale = packed_scale_of<PG>(vs, b / 2);
-      const f16x2 s01 = f16x2{half_of(scale, 0), half_of(scale, 1)} * sixteenth;
-      const f16x2 s23 = f16x2{half_of(scale, 2), half_of(scale, 3)} * sixteenth;
+      const f16x2 s01 = f16x2{half_of(scale, 0), half_of(scale, 1)};
+      const f16x2 s23 = f16x2{half_of(scale, 2), half_of(scale, 3)};
       unsigned w[4];
-      whole_values(vw[b], f16x2{half_of(scale, 4), half_of(scale, 5)}, f16x2{half_of(scale, 6), half_of(scale, 7)}, w);
+      whole_values<true>(vw[b], f16x2{half_of(scale, 4), half_of(scale, 5)} * sixteenth,
+                         f16x2{half_of(scale, 6), half_of(scale, 7)} * sixteenth, w);
       typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
 #pragma unroll
       for (int i = 0; i < 2; ++i)                  // elements 32 b + r, 32 b + 16 + r
