@@ -169,14 +169,15 @@ struct PackedLift {
   f16x2 by[2];             // of this lane's word
   __device__ __forceinline__ static PackedLift none(int lane) { return at(0, lane); }
   __device__ __forceinline__ static PackedLift at(int exponent, int lane) {
-    // 2^(29 - exponent), -1 to 29, as 2^half and 2^(the rest)
+    // 2^(29 - exponent), -1 to 29, as 2^half and 2^(the rest): scalars, by their fields
     const int up = 29 - exponent, half = up >> 1;
+    const unsigned a = (unsigned)(15 + half) * 0x04000400u, b = (unsigned)(15 + up - half) * 0x04000400u, one = 0x3c003c00u;
     const bool bias = lane % 4 >= 2;
-    const _Float16 one = (_Float16)1.f;
-    const _Float16 a = bias ? one : (_Float16)ldexpf(1.f, half), b = bias ? one : (_Float16)ldexpf(1.f, up - half);
-    return PackedLift{exponent, {f16x2{a, a}, f16x2{b, b}}};
+    return PackedLift{exponent, {__builtin_bit_cast(f16x2, bias ? one : a), __builtin_bit_cast(f16x2, bias ? one : b)}};
   }
-  __device__ __forceinline__ float down() const { return ldexpf(1.f, exponent - 29); }
+  // 2^n for -126 <= n <= 127, a scalar where n is.
+  __device__ __forceinline__ static float power(int n) { return __uint_as_float((unsigned)(127 + n) << 23); }
+  __device__ __forceinline__ float down() const { return power(exponent - 29); }
   __device__ __forceinline__ unsigned raised(unsigned word) const {
     return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, word) * by[0] * by[1]);
   }
@@ -313,9 +314,11 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, WIDE>& t, const Pac
     const int word = threadIdx.x % 4;
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      const int key = kb + blk * 16 + g * 4 + word * 2;
-      auto there = [&](int k) { return b.page[blk] >= 0 && k <= t.last && (k >= t.first || k < t.keep); };
-      if (word < 2) steps[blk] &= (there(key) ? 0xffffu : 0u) | (there(key + 1) ? 0xffff0000u : 0u);
+      const int key = kb + blk * 16 + g * 4 + word * 2, last = b.page[blk] >= 0 ? t.last : -1;
+      unsigned there = (key <= last ? 0xffffu : 0u) | (key < last ? 0xffff0000u : 0u);
+      if (kb < t.first)
+        there &= (key >= t.first || key < t.keep ? 0xffffu : 0u) | (key + 1 >= t.first || key + 1 < t.keep ? 0xffff0000u : 0u);
+      steps[blk] &= word < 2 ? there : ~0u;
     }
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk)
@@ -343,11 +346,18 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, WIDE>& t, const Pac
   const int top = max((int)top2[0], (int)top2[1]);
   float change = corr;
   if (__builtin_amdgcn_ballot_w64(top >= (t.lift.exponent + 1) << 10) != 0) {
-    int exponent = 0;
-#pragma unroll
-    for (int bit = 16; bit > 0; bit >>= 1)
-      if (__builtin_amdgcn_ballot_w64(top >= (exponent + bit) << 10) != 0) exponent += bit;
-    change *= ldexpf(1.f, t.lift.exponent - exponent);
+    // (the largest of sixteen lanes in each, then of the four sixteens as scalars)
+    int most = top;
+    auto with = [&](auto how) {
+      most = max(most, __builtin_amdgcn_update_dpp(0, most, decltype(how)::value, 0xf, 0xf, true));
+    };
+    with(std::integral_constant<int, 0xB1>{});
+    with(std::integral_constant<int, 0x4E>{});
+    with(std::integral_constant<int, 0x141>{});
+    with(std::integral_constant<int, 0x140>{});
+    const int exponent = max(max(__builtin_amdgcn_readlane(most, 0), __builtin_amdgcn_readlane(most, 16)),
+                             max(__builtin_amdgcn_readlane(most, 32), __builtin_amdgcn_readlane(most, 48))) >> 10;
+    change *= PackedLift::power(t.lift.exponent - exponent);
     t.lift = PackedLift::at(exponent, threadIdx.x % kWave);
   }
   // (far into a context most blocks bring no new largest score)
@@ -401,15 +411,13 @@ __device__ __forceinline__ void packed_update(PackedTile<NB, WIDE>& t, const Pac
   }
 }
 
-// The rows' sums with what the zeros take off, or with the second parts, as often as they count.
+// The rows' sums with what the zeros take off, or with the second parts; o counts as often as the lift says still.
 template <int NB, bool WIDE>
 __device__ __forceinline__ void packed_finish(PackedTile<NB, WIDE>& t) {
-  const float down = t.lift.down();
 #pragma unroll
   for (int db = 0; db < 2 * NB; ++db)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      t.o[db][j] = down * (WIDE ? fmaf(t.oz[db][j], 1.f / 2048.f, t.o[db][j]) : t.o[db][j] + t.oz[db / 4][j]);
+    for (int j = 0; j < 4; ++j) t.o[db][j] = WIDE ? fmaf(t.oz[db][j], 1.f / 2048.f, t.o[db][j]) : t.o[db][j] + t.oz[db / 4][j];
   t.l = col4_sum(t.l);
 }
 
@@ -543,6 +551,7 @@ __global__ __launch_bounds__((PackedShape<NB, WIDE>::THREADS), packed_waves(NB, 
   typedef float Stats[16][2];
   Results* s_o = (Results*)packed_lds;
   Stats* s_ml = (Stats*)(packed_lds + WAVES * 16 * Shape::ROW);
+  __shared__ float s_down[WAVES];
   __shared__ unsigned s_before[2];
   __shared__ int s_plan[5];
   const AttentionArgs& a = args.base;
@@ -615,6 +624,7 @@ __global__ __launch_bounds__((PackedShape<NB, WIDE>::THREADS), packed_waves(NB, 
       s_ml[wave][r][0] = t.m;
       s_ml[wave][r][1] = t.l;
     }
+    if (lane == 0) s_down[wave] = t.lift.down();
 #pragma unroll
     for (int db = 0; db < DB; ++db) *(f32x4*)&s_o[wave][r][db * 16 + g * 4] = t.o[db];
     __syncthreads();
@@ -639,7 +649,7 @@ __global__ __launch_bounds__((PackedShape<NB, WIDE>::THREADS), packed_waves(NB, 
       for (int w = 0; w < WAVES; ++w) {
         const float ww = __builtin_amdgcn_exp2f(s_ml[w][row][0] - Mc);
         sum = fmaf(s_ml[w][row][1], ww, sum);
-        acc = fmaf(s_o[w][row][d], ww, acc);
+        acc = fmaf(s_o[w][row][d], ww * s_down[w], acc);
       }
       if (whole) {
         sum = sum_with_sink(sum, M, a.sink, sink_of(row));
@@ -753,7 +763,7 @@ __global__ __launch_bounds__(256, packed_waves(NB, WIDE)) void packed_walk_kerne
   }
   packed_finish<NB, WIDE>(t);
   if (!row_ok) return;
-  const float sum = sum_with_sink(t.l, t.m, a.sink, head), inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float sum = sum_with_sink(t.l, t.m, a.sink, head), inv = sum > 0.f ? t.lift.down() / sum : 0.f;
   typedef T four __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int db = 0; db < DB; ++db) {
