@@ -3,11 +3,29 @@
 // The sum is a whole number in 32 bits, exact and the same in whatever order it is made (K up to 131,072:
 // 127 x 127 x K < 2^31); it becomes a float32 number, then the weight's
 // scale follows, then the row's (rows near float32's largest number stay finite where the result is).  PAIR: W is [2, N, K], gate
-// rows, then up rows, and C = unit(gate, up) (gated_unit) of the scaled sums, which are not rounded to the output's type first.
+// rows, then up rows, and C = unit(gate, up) (Int8Unit) of the scaled sums, which are not rounded to the output's type first.
 #pragma once
 #include "gemm_common.h"
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
+
+// The gated unit of all these products: gated_unit's three forms in one, by the hardware's exp2 and reciprocal (an ulp each),
+// the same instructions whichever kernel a row's product comes from, so that its bits do not depend on the rows beside it.
+// (The clamps change nothing without a limit; a clamp takes NaN for its limit, as gated_unit's does.)
+struct Int8Unit {
+  float top, lift, slope, cubic;
+  __device__ __forceinline__ explicit Int8Unit(float limit) {
+    const bool clamped = limit > 0.f, gelu = limit < 0.f;
+    top = clamped ? limit : INFINITY, lift = clamped ? 1.f : 0.f;
+    // the weight exp2(g (slope + cubic g^2)): of the sigmoid, or for gelu_tanh(g) = g sigmoid(2 sqrt(2 / pi) (g + 0.044715 g^3))
+    slope = (clamped ? -1.702f : gelu ? -2.f * 0.79788456080286536f : -1.f) * 1.44269504f;
+    cubic = gelu ? 0.044715f * slope : 0.f;
+  }
+  __device__ __forceinline__ float operator()(float gate, float up) const {
+    const float g = fminf(gate, top), u = fminf(fmaxf(up, -top), top) + lift;
+    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * fmaf(cubic, g * g, slope))) * u;
+  }
+};
 
 struct Int8Args {
   const signed char* a;      // [M, row]

@@ -29,12 +29,13 @@ __device__ __forceinline__ void finish_few(const Int8Args& a, i32x4 (&acc)[HALVE
   const int n = n0 + lane / 16 * 4;
   if (n >= a.N || m >= a.M) return;
   const float row = scales[m];
+  const Int8Unit unit(a.limit);
   f32x4 v;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int column = min(n + i, a.N - 1);
     v[i] = (float)acc[0][i] * a.w_scale[column] * row;
-    if constexpr (PAIR) v[i] = gated_unit(v[i], (float)acc[1][i] * a.w_scale[a.N + column] * row, a.limit);
+    if constexpr (PAIR) v[i] = unit(v[i], (float)acc[1][i] * a.w_scale[a.N + column] * row);
   }
   store4<TC>((TC*)a.c + (int64_t)m * a.N + n, v, a.N - n);
 }

@@ -679,6 +679,7 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
       }
     }
     constexpr int COLS = PAIR ? TN / 2 : TN;
+    const Int8Unit unit(g.limit);
     auto scales = [&](const float* p, int n) {
       f32x4 s;
 #pragma unroll
@@ -701,11 +702,7 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           v[e] = (float)acc[tn][tm][e] * s0[e] * row;
-          if constexpr (PAIR) {
-            const float up = (float)acc[tn + TN / 2][tm][e] * s1[e] * row;
-            const float gc = fminf(v[e], top), uc = fminf(fmaxf(up, -top), top) + lift;
-            v[e] = gc * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(gc * fmaf(cubic, gc * gc, slope))) * uc;
-          }
+          if constexpr (PAIR) v[e] = unit(v[e], (float)acc[tn + TN / 2][tm][e] * s1[e] * row);
         }
         store4<TO>(c + (int64_t)m * g.N + n, v, g.N - n);
       }
