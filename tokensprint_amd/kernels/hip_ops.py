@@ -207,12 +207,15 @@ class HipOps:
 
     def reset_scratch(self) -> None:
         """Put what this provider keeps between calls back to its start: the arrival counts
-        of the decode kernel's own merge at zero.  Called after a failed call, and by the
-        engine before its warm-up step and before graphs are captured."""
+        of the decode kernel's own merge at zero, and of those that `_counts` gives the current
+        stream's (another stream's may be counted in at this moment, and a graph makes its own
+        zeros).  Called after a failed call, and by the engine before its warm-up step and before
+        graphs are captured."""
         self._arrivals.zero_()
-        if self._raw_stream(self._device_index) == 0 or not torch.cuda.is_current_stream_capturing():
-            for counts in self._count_arrays.values():
-                counts.zero_()
+        stream = self._raw_stream(self._device_index)
+        counts = self._count_arrays.get((stream, 0))
+        if counts is not None and not (stream and self.lib.ts_capture_id(c_void_p(stream))):
+            counts.zero_()
 
     def _counts(self, n):
         """At least `n` zeros in which workgroups count themselves in, left as zeros by every
