@@ -1580,7 +1580,7 @@ class HipOps:
             cache.v_pages.data_ptr(), batch.positions.data_ptr(), batch.entry_of_token.data_ptr(),
             batch.q_start.data_ptr(), batch.ctx_len.data_ptr(), table.data_ptr(), table.shape[1], T,
             batch.num_entries, num_heads, num_kv_heads, head_dim, cache.page_size, cache.num_pages,
-            0 if window is None else int(window), scale)
+            0 if window is None else min(int(window), (1 << 31) - 1), scale)   # (further than any sequence goes)
 
     # ------------------------------------------------------------ sampling
     def argmax(self, logits):
