@@ -85,3 +85,67 @@ def test_steps_keep_their_bits(ops, gpu_device, hd):
     # at the most, 2e-3 of a weight, independent)
     worst = relative(got, want)
     assert worst <= 2.0 ** -8 + 2.0 ** -9
+
+
+def one_channel_keys(whole, nkv, hd, device, seed, scores=None):
+    """Keys of one element, which is the score that a query of one element gives (in 11 bits)."""
+    k = torch.zeros(whole.num_tokens, nkv, hd, dtype=BF16, device=device)
+    k[:, :, 0] = (rand((whole.num_tokens, nkv), F32, device, seed) + (0 if scores is None else scores[:, None])).to(BF16)
+    return k
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("std", [3e-6, 1e-5, 1e-4, 1.0, 30.0, 3e3, 1e5])
+def test_values_of_any_size(ops, gpu_device, hd, std):
+    """From steps of a few of float16's smallest numbers to its largest."""
+    batch, whole, table, cache = scene(gpu_device, nkv=2, hd=hd, page=16, spans=[(700, 40), (0, 33)])
+    k = one_channel_keys(whole, 2, hd, gpu_device, 1)
+    v = (rand((whole.num_tokens, 2, hd), F32, gpu_device, 2) * std).to(BF16)
+    q = torch.zeros(batch.num_tokens, 4, hd, dtype=BF16, device=gpu_device)
+    q[:, :, 0] = 8.0
+    got, want = run(ops, q, k, v, batch, whole, table, cache, 2)
+    # (and scores of up to 4 to 2^-11 of themselves, independent of each other: 2^-9 at the most)
+    worst = relative(got, want)
+    assert worst <= TOLERANCE[BF16] + 2.0 ** -9
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("std", [1e-5, 1e-3, 1.0, 300.0, 3e4])
+def test_keys_of_any_size(ops, gpu_device, hd, std):
+    """With queries that bring the scores back to ordinary ones."""
+    batch, whole, table, cache = scene(gpu_device, nkv=2, hd=hd, page=16, spans=[(700, 40), (0, 33)])
+    k = (rand((whole.num_tokens, 2, hd), F32, gpu_device, 1) * std).to(BF16)
+    v = rand((whole.num_tokens, 2, hd), BF16, gpu_device, 2)
+    q = (rand((batch.num_tokens, 4, hd), F32, gpu_device, 3) * (8 / hd ** 0.5 / std)).to(BF16)
+    got, want = run(ops, q, k, v, batch, whole, table, cache, 2)
+    # (hd independent roundings of 2^-11 |k q|: scores, of a deviation of 1, to 2^-9 at the most)
+    worst = relative(got, want)
+    assert worst <= TOLERANCE[BF16] + 2.0 ** -9
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed", "one large block"])
+@pytest.mark.parametrize("sets", [1, 2])
+def test_values_of_many_sizes_in_one_context(ops, gpu_device, hd, order, sets):
+    """Blocks of 16 tokens whose steps lie on either side of every border between scales; scores fall by ln 2 for every
+    doubling, so that all tokens bring about as much to the sum."""
+    spans = [(1500, 40), (0, 33)] if sets == 2 else [(1500, 2), (90, 30)] + [(33 + i, 1) for i in range(130)]
+    batch, whole, table, cache = scene(gpu_device, nkv=2, hd=hd, page=16, spans=spans)
+    n = whole.num_tokens
+    exponent = torch.linspace(-12, 17, n, device=gpu_device).round()
+    if order == "falling":
+        exponent = exponent.flip(0)
+    elif order == "mixed":
+        exponent = exponent[torch.randperm(n, generator=torch.Generator().manual_seed(5)).to(gpu_device)]
+    elif order == "one large block":
+        exponent = torch.full_like(exponent, -9)
+        exponent[48:64] = 16
+    k = one_channel_keys(whole, 2, hd, gpu_device, 1, -0.6931 * exponent)
+    v = (rand((n, 2, hd), F32, gpu_device, 2) * torch.exp2(exponent)[:, None, None]).clamp(-6e5, 6e5).to(BF16)
+    q = torch.zeros(batch.num_tokens, 4, hd, dtype=BF16, device=gpu_device)
+    q[:, :, 0] = 8.0
+    got, want = run(ops, q, k, v, batch, whole, table, cache, 2)
+    # (scores of up to 12 + 4 to 2^-11 of themselves, independent of each other: 2^-7 at the most for any one weight,
+    # a third of that as the deviation of all of them, twice that is allowed)
+    worst = relative(got, want)
+    assert worst <= TOLERANCE[BF16] + 2.0 ** -7 * 2 / 3

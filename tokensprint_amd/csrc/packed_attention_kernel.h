@@ -55,12 +55,11 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
 // Eight codes as the numbers 16 + c: codes 0 and 4, 1 and 5, 2 and 6, 3 and 7 of a word of keys (bfloat16) or of
-// values (float16); SIXTEENTHS (float16 only): as 1 + c / 16.
-template <bool VALUES, bool SIXTEENTHS = false>
+// values (float16).
+template <bool VALUES>
 __device__ __forceinline__ void packed_codes(unsigned word, unsigned (&out)[4]) {
   // (one of the two constants in a vector register, one in a scalar: `and` and `or` are one instruction then)
-  unsigned bits = VALUES ? 0x03c003c0u : 0x00780078u;
-  unsigned lead = SIXTEENTHS ? 0x3c003c00u : VALUES ? 0x4c004c00u : 0x41804180u;
+  unsigned bits = VALUES ? 0x03c003c0u : 0x00780078u, lead = VALUES ? 0x4c004c00u : 0x41804180u;
   asm("" : "+v"(bits));
   asm("" : "+s"(lead));
   out[0] = (word & bits) | lead;
@@ -68,21 +67,18 @@ __device__ __forceinline__ void packed_codes(unsigned word, unsigned (&out)[4]) 
   out[2] = ((VALUES ? __builtin_amdgcn_alignbit(word, word, 8) : word >> 8) & bits) | lead;
   out[3] = (__builtin_amdgcn_alignbit(word, word, 12) & bits) | lead;
 }
-// The whole numbers code - zero of a word of keys in float16, with the bias of their token; SIXTEENTHS: a
-// sixteenth of each, with a sixteenth of the bias (exact too).
-template <bool SIXTEENTHS = false>
+// The whole numbers code - zero of a word of keys in float16, with the bias of their token.
 __device__ __forceinline__ void whole_keys(unsigned word, _Float16 bias, unsigned (&out)[4]) {
   unsigned c[4];
-  packed_codes<true, SIXTEENTHS>(__builtin_amdgcn_alignbit(word, word, 32 - (kPackTurnV - kPackTurnK)), c);
+  packed_codes<true>(__builtin_amdgcn_alignbit(word, word, 32 - (kPackTurnV - kPackTurnK)), c);
   const f16x2 b = {bias, bias};
 #pragma unroll
   for (int i = 0; i < 4; ++i) out[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, c[i]) + b);
 }
 // The same of a word of values, with the biases of tokens 0 and 1, 2 and 3.
-template <bool SIXTEENTHS = false>
 __device__ __forceinline__ void whole_values(unsigned word, f16x2 b01, f16x2 b23, unsigned (&out)[4]) {
   unsigned c[4];
-  packed_codes<true, SIXTEENTHS>(word, c);
+  packed_codes<true>(word, c);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     out[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, c[i]) + (i % 2 ? b23 : b01));

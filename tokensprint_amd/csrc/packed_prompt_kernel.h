@@ -1,21 +1,33 @@
 // Prompts' attention over keys and values of 4 bits: 32 query rows a wavefront, four wavefronts an item, as over a
 // cache of bfloat16 (attention_prefill_tall_kernel.h), whose tiles in LDS are made here from a turn's codes: head sizes 64 and 128.
 //
-// A turn is 64 keys, four blocks of a page; a wavefront turns one block's codes into float16 numbers step (code - zero) / 16
-// and writes them where its operands are read, 15 instructions for eight of them, once for the 128 rows of an item. The
-// sixteenth keeps every number in float16's range; queries are float16 as well, scaled by a power of two a row (their
-// bfloat16 bits are exact then), and so are weights, which count 2^15 times: as they are, 9 below the row's largest score
-// they would have fewer than 11 bits, and 17 below none (4,000 keys 14 below one of no value: 0.6 % of the result; now
-// bits go from 20 below on).  What is rounded is a key's or a value's number, to 11 bits (a score s that one element
-// makes alone is off by 2^-11 s at the most), and to 2^-21 where it is below 2^-10: a 32nd of a step of 2^-16.  (As
+// A turn is 64 keys, four blocks of a page; a wavefront turns one block's codes into float16 numbers step (code - zero)
+// and writes them where its operands are read, once for the 128 rows of an item.  Numbers count a power of two times, so
+// that they stand high in float16's range (PromptScale); queries are float16 as well, scaled by a power of two a row
+// (their bfloat16 bits are exact then), and so are weights, which count 2^15 times: as they are, 9 below the row's largest
+// score they would have fewer than 11 bits, and 17 below none (4,000 keys 14 below one of no value: 0.6 % of the result;
+// now bits go from 20 below on).  What is rounded is a key's or a value's number, to 11 bits (a score s that one element
+// makes alone is off by 2^-11 s at the most).  (As
 // step (16 + code) less a rounded step (16 + zero), in 4 instructions less, results were three times as far off.)
 // The next turn's codes, asked for a turn ahead, become numbers between the scores' products, a word a step, and the second
 // half of a turn's weights are made between the first half's products: a turn is one meeting of the workgroup.
-// 4,096 tokens behind 4,096, 32 heads of 128 over 8: 470 us, 880 TFLOP/s (all codes of a turn first, then its products 483; over
-// a cache of bfloat16 423), vector instructions three quarters of the time and matrix instructions 40 %.
+// 4,096 tokens behind 4,096, 32 heads of 128 over 8: 475 to 495 us by card, 835 to 870 TFLOP/s (all codes of a turn first, then
+// its products: 0.6 % longer; over a cache of bfloat16 a tenth shorter), vector instructions three quarters of the time and
+// matrix instructions 40 %.
 #pragma once
 #include "attention_prefill_tall_kernel.h"
 #include "packed_attention_kernel.h"
+
+// What a block's numbers count: values 2^11 times where its largest step is below 2, else 2^-4, keys 2^4 times below 256,
+// else 2^-4: 15 steps stay below float16's largest number, and a step of float16's smallest has 11 bits in a block of the
+// first kind (in one of the second numbers are held to 2^-21).  Nearly every block is of the first; one of the second is
+// told to the workgroup beside the tile, and the scores and weights of a turn with such a block make up for it.
+// (A sixteenth for all, the most that holds the largest step, took 1.7 % less time and left numbers below 2^-10 without all
+// their bits: values of 1e-4 came out 0.3 % off, of 1e-5 3 %.)
+struct PromptScale {
+  static constexpr int kValues = 11, kKeys = 4, kLarge = -4;
+  static constexpr int kLargeValues = 1, kLargeKeys = 2;               // a block's flags
+};
 
 // Tiles and operands lie as there. SETS sets of four wavefronts split an item's turns and merge through LDS at the end.
 template <int HD, int SETS, bool EXTRA>
@@ -25,9 +37,11 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
   constexpr int SUB = HD / 32;                 // slots of 1 KB per sixteen keys
   constexpr int VALUES = KEYS * HD * 2;        // bytes of a turn's keys; its values lie behind them
   constexpr int BUF = 2 * VALUES;
-  constexpr float kUp = 15.f;                  // weights, their sums and o count 2^kUp times, values' numbers a sixteenth
+  constexpr float kUp = 15.f;                  // weights and their sums count 2^kUp times
   static_assert((HD == 64 || HD == 128) && G == TILES, "rows of 128 or 256 bytes, a block a wavefront");
   extern __shared__ __attribute__((aligned(1024))) unsigned char prefill_lds[];
+  __shared__ int s_flags[SETS][2][TILES], s_any[SETS];     // PromptScale's, of the rings' blocks; whether there are any
+  __shared__ float s_down[SETS][TILES];
   const AttentionArgs& a = args.base;
   const int wave_all = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int wave = wave_all % TILES, set = SETS == 1 ? 0 : wave_all / TILES;
@@ -65,8 +79,8 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
   const int hh = hb * 16 + c % 16 % args.rows_per_token;
   const int head = kvh * group + min(hh, group - 1);
   const bool row_ok = in16 < tq && ti < ntok && hh < group;
-  // the query row in float16, its largest magnitude brought to 2^13 .. 2^14; `back`: what that and the sixteenth of the
-  // keys' numbers take out of a product
+  // the query row in float16, its largest magnitude brought to 2^13 .. 2^14; `back`: what takes that and the keys' 2^4
+  // out of a product
   f16x8 q[KS];
   float back;
   {
@@ -84,7 +98,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     }
     top = halves_max(top);
     const int up = top > 0.f && top < INFINITY ? min(14 - __builtin_amdgcn_frexp_expf(top), 120) : 0;
-    back = ldexpf(16.f, -up);
+    back = ldexpf(1.f, -PromptScale::kKeys - up);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -126,8 +140,10 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
   fetch_id(kb_first);
   unsigned kw[NB], vw[NB], vs;
   unsigned ks[PG], kz[PG];
+  int held;                                          // the first key of the block that they are of
   auto issue = [&](int j) {
-    const int v = kb_first + KEYS * SETS * j, in = (walk.real(v) + 16 * wave) & (P - 1);
+    const int v = kb_first + KEYS * SETS * j, at_key = walk.real(v) + 16 * wave, in = at_key & (P - 1);
+    held = next_page < 0 ? 1 << 30 : at_key;
     const int64_t at = (((int64_t)max(next_page, 0) * a.nkv + kvh) * P + in) / 16 * BYTES;
     const unsigned char* kp = (const unsigned char*)a.k_pages + at;
     const unsigned char* vp = (const unsigned char*)a.v_pages + at;
@@ -141,17 +157,52 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     }
     fetch_id(v + KEYS * SETS);
   };
-  // Codes into the tile, a word of a lane's at a time (keys, then values): 1 + c / 16, less 1 + zero / 16 (exact), times the step.
-  // (The sixteenth on the step instead cost steps below 2^-10 their last bits, for every number of a group: at
-  // 2^-14 four of eleven, and results were 0.8 % off.)
+  // Of the item's last turn: steps that a page holds of nobody's keys are none, and have no say in scales.
+  auto mask_steps = [&]() {
+    const int key = held + g4 * 4 + lane % 4 * 2;
+    const unsigned there = (key <= pos_last ? 0xffffu : 0u) | (key < pos_last ? 0xffff0000u : 0u);
+    vs &= lane % 4 < 2 ? there : ~0u;
+#pragma unroll
+    for (int i = 0; i < PG; ++i) ks[i] = held + r16 <= pos_last ? ks[i] : 0u;
+  };
+  // Steps as the numbers want them, keys', then values', and the block's flags.  (Without a branch, which would end the
+  // stretch in which the compiler may order products and these.)
+  const unsigned step_lanes = lane % 4 < 2 ? 0x40004000u : 0u;         // bit 14: 2 and more
+  int flags_now = 0, told = 0;
+  // (of their own: in the registers that loads go to, they would make the next turn's be waited for)
+  _Float16 key_step[PG];
+  unsigned value_steps = 0;
+  auto scale_keys = [&]() {
+    unsigned top = ks[0];
+#pragma unroll
+    for (int i = 1; i < PG; ++i) top = max(top, ks[i]);
+    const bool large = __builtin_amdgcn_ballot_w64(top >= 0x5c00u) != 0;          // 256
+    const _Float16 up = __builtin_bit_cast(_Float16, (unsigned short)(large ? 0x2c00u : 0x4c00u));
+    flags_now = large ? PromptScale::kLargeKeys : 0;
+#pragma unroll
+    for (int i = 0; i < PG; ++i)
+      key_step[i] = __builtin_bit_cast(_Float16, (unsigned short)ks[i]) * up;
+  };
+  auto scale_values = [&]() {
+    const bool large = __builtin_amdgcn_ballot_w64((vs & step_lanes) != 0) != 0;
+    flags_now += large ? PromptScale::kLargeValues : 0;
+    const unsigned up = step_lanes != 0 ? (large ? 0x2c002c00u : 0x68006800u) : 0x3c003c00u;
+    value_steps = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, vs) * __builtin_bit_cast(f16x2, up));
+  };
+  // (a wavefront that has told of a block once does so for all that follow, so that what stands there is this turn's)
+  auto tell = [&](int* flags) {
+    if ((flags_now | told) == 0) return;
+    told = 1;
+    flags[wave] = flags_now;
+    s_any[set] = 1;
+  };
+  // Codes into the tile, a word of a lane's at a time (keys, then values): 16 + c, less 16 + zero (exact), times the step.
   auto unpack = [&](unsigned char* buf, int n) {
-    const _Float16 sixteenth = (_Float16)0.0625f;
     if (n < NB) {
       const int b = n;
       unsigned w[4];
-      whole_keys<true>(kw[b], __builtin_bit_cast(_Float16, (unsigned short)kz[b / 2]) * sixteenth, w);
-      const _Float16 s1 = __builtin_bit_cast(_Float16, (unsigned short)ks[b / 2]);
-      const f16x2 s = {s1, s1};
+      whole_keys(kw[b], __builtin_bit_cast(_Float16, (unsigned short)kz[b / 2]), w);
+      const f16x2 s = {key_step[b / 2], key_step[b / 2]};
       u32x4 out;
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, w[i]) * s);
@@ -160,12 +211,11 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
       *(u32x4*)(buf + (piece ^ (64 * b))) = out;
     } else {
       const int b = n - NB;
-      const u32x4 scale = packed_scale_of<PG>(vs, b / 2);
+      const u32x4 scale = packed_scale_of<PG>(value_steps, b / 2);
       const f16x2 s01 = f16x2{half_of(scale, 0), half_of(scale, 1)};
       const f16x2 s23 = f16x2{half_of(scale, 2), half_of(scale, 3)};
       unsigned w[4];
-      whole_values<true>(vw[b], f16x2{half_of(scale, 4), half_of(scale, 5)} * sixteenth,
-                         f16x2{half_of(scale, 6), half_of(scale, 7)} * sixteenth, w);
+      whole_values(vw[b], f16x2{half_of(scale, 4), half_of(scale, 5)}, f16x2{half_of(scale, 6), half_of(scale, 7)}, w);
       typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
 #pragma unroll
       for (int i = 0; i < 2; ++i)                  // elements 32 b + r, 32 b + 16 + r
@@ -175,6 +225,8 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     }
   };
   auto unpack_all = [&](unsigned char* buf) {
+    scale_keys();
+    scale_values();
 #pragma unroll
     for (int n = 0; n < 2 * NB; ++n) unpack(buf, n);
   };
@@ -185,9 +237,11 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
   float m = -INFINITY, l = 0.f;      // l: this lane's share of the row's sum
+  int up_o = PromptScale::kValues;   // o counts 2^(kUp + up_o) times: as the least of the blocks' values so far
 
   static_assert(KS == 2 * NB, "a word to unpack for every step of the scores");
-  auto work = [&](int j, int kb, const unsigned char* buf, unsigned char* next) {
+  auto work = [&](int j, int kb, const unsigned char* buf, unsigned char* next, const int* flags) {
+    const int any = s_any[set];
     // a step's operands are asked for ahead of its products
     constexpr int AHEAD = 2;
     f16x8 kf[AHEAD][B];
@@ -210,6 +264,8 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
       for (int b = 0; b < B; ++b)
         st[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[s % AHEAD][b], q[s], st[b], 0, 0, 0);
       if (s + AHEAD < KS) read_keys(s + AHEAD);
+      if (s == 0) scale_keys();
+      if (s == 1) scale_values();
       unpack(next, s);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -221,8 +277,18 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     };
     read_values(0), read_values(1);
     __builtin_amdgcn_sched_barrier(0);
+    const bool other = uniform(any) != 0;
+    // keys that count 2^-4 times: their products as the others'
+    auto even_keys = [&]() {
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          st[b][i] *= uniform(flags[2 * b + i / 8]) & PromptScale::kLargeKeys ? 256.f : 1.f;
+    };
     const int at = kb + 8 * h;       // register i of block b: key at + 32 b + 16 (i / 8) + i % 8
     if (EXTRA) {
+      if (other) even_keys();
       if (x.capped) {
 #pragma unroll
         for (int b = 0; b < B; ++b)
@@ -242,8 +308,9 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
       }
       scale_log2 = 1.f;
     }
-    if (!(kb + KEYS - 1 <= tile_first && kb >= tile_lo_last)) {
+    if (!(kb + KEYS - 1 <= tile_first && kb >= tile_lo_last) || (!EXTRA && other)) {
       asm volatile("" ::: "memory");   // keeps this a branch
+      if (!EXTRA && other) even_keys();
       // (a key's number is a constant beyond the lane's first: the row's bounds are brought
       // there once a turn, so no register holds a key's)
       const int last = row_pos - at, lowest = row_lo - at, kept = a.keep - at;
@@ -273,18 +340,48 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
         for (int i = 0; i < 16; ++i) o[db][i] *= corr;
     }
     const float rise = kUp - max2(m, -1e30f);
+    float by = scale_log2;
+    unsigned ones[G];                // what two weights count in the row's sum, which knows no scales
+#pragma unroll
+    for (int g = 0; g < G; ++g) ones[g] = 0x3c003c00u;
+    if (other) {
+      asm volatile("" ::: "memory");
+      int up[G], least = up_o;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        up[g] = uniform(flags[g]) & PromptScale::kLargeValues ? PromptScale::kLarge : PromptScale::kValues;
+        least = min(least, up[g]);
+      }
+      if (least != up_o) {
+        const float change = PackedLift::power(least - up_o);
+        up_o = least;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[db][i] *= change;
+      }
+      // (weights of 2^-n: scores less by n)
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        ones[g] = (unsigned)(15 + up[g] - up_o) * 0x04000400u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          st[g / 2][g % 2 * 8 + i] = fmaf(st[g / 2][g % 2 * 8 + i], by, (float)(up_o - up[g]));
+      }
+      by = 1.f;
+    }
     // the first block's weights, then its values' products between those of the second
     f16x8 pv[G];
     // (the row's sum is of the weights as they enter the products, two at a time)
     float before = 0.f;
     auto weight = [&](int b, int i) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][i], scale_log2, rise));
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][i], by, rise));
       if (i % 2 == 0) {
         before = p;
         return;
       }
       const f16x2 two = {(_Float16)before, (_Float16)p};
-      l = __builtin_amdgcn_fdot2(two, f16x2{(_Float16)1.f, (_Float16)1.f}, l, false);
+      l = __builtin_amdgcn_fdot2(two, __builtin_bit_cast(f16x2, ones[2 * b + i / 8]), l, false);
       pv[2 * b + i / 8][i % 8 - 1] = two[0], pv[2 * b + i / 8][i % 8] = two[1];
     };
     auto product = [&](int g, int db) { o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[g][db], pv[g], o[db], 0, 0, 0); };
@@ -307,15 +404,20 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+  if (lane == 0) s_flags[set][0][wave] = s_flags[set][1][wave] = s_any[set] = 0;
+  meet();
   if (mine > 0) {
     issue(0);
+    if (held + 15 > pos_last) mask_steps();
     unpack_all(ring);
+    tell(s_flags[set][0]);
     if (mine > 1) issue(1);
   }
   meet();
   for (int j = 0; j < rounds; ++j) {
     const int kb = walk.real(kb_first + KEYS * SETS * j);
     unsigned char *buf = ring + (j & 1) * BUF, *next = ring + (~j & 1) * BUF;
+    if (j + 1 < mine && held + 15 > pos_last) mask_steps();
     // (behind the last turn what is left in the registers once more, into a tile that nobody reads)
     const bool seen = kb <= tile_last && (kb + KEYS - 1 >= tile_lo || kb < a.keep);
     if (j < mine && !seen) {
@@ -323,7 +425,8 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
       if (j + 2 < mine) issue(j + 2);
     }
     asm volatile("" ::: "memory");             // (one branch and another: as the two ways of one, the sums would be moved)
-    if (j < mine && seen) work(j, kb, buf, next);
+    if (j < mine && seen) work(j, kb, buf, next, s_flags[set][j & 1]);
+    tell(s_flags[set][~j & 1]);
     meet();
   }
 
@@ -345,7 +448,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
   };
   if constexpr (SETS == 1) {
     const float sum = sum_with_sink(l, m, a.sink, head);
-    const float inv = sum > 0.f ? 0x1p-11f / sum : 0.f;
+    const float inv = sum > 0.f ? PackedLift::power(-15 - up_o) / sum : 0.f;
 #pragma unroll
     for (int u = 0; u < 2 * DB; ++u) {
       float v[8];
@@ -365,6 +468,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     for (int i = 0; i < REGS; ++i) lds_o[(wave_all * REGS + i) * kWave + lane] = o[i / 16][i % 16];
     lds_ml[wave_all * 2 * kWave + lane] = m;
     lds_ml[(wave_all * 2 + 1) * kWave + lane] = l;
+    if (lane == 0) s_down[set][wave] = PackedLift::power(-15 - up_o);
     __syncthreads();
     float ms[SETS], w[SETS], m_use = -1e30f, sum = 0.f;
 #pragma unroll
@@ -377,9 +481,10 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
       // (a set that saw no key of this row has m = -inf and weight 0)
       w[s] = __builtin_amdgcn_exp2f(ms[s] - m_use);
       sum += lds_ml[((s * TILES + wave) * 2 + 1) * kWave + lane] * w[s];
+      w[s] *= s_down[s][wave];
     }
     sum = sum_with_sink(sum, m_use, a.sink, head);
-    const float inv = sum > 0.f ? 0x1p-11f / sum : 0.f;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll
     for (int n = 0; n < UNITS; ++n) {
       const int u = set * UNITS + n;
@@ -403,7 +508,7 @@ static int launch_packed_prompt_of(const PackedArgs& args, hipStream_t stream) {
   const int heads = args.base.nkv * args.head_blocks;
   constexpr int rings = SETS * 2 * KEYS * HD * 4, merge = SETS == 1 ? 0 : SETS * TILES * (HD / 2 + 2) * kWave * 4;
   constexpr int lds = rings > merge ? rings : merge;
-  static_assert(lds <= 160 * 1024, "LDS of a compute unit");
+  static_assert(lds + 1024 <= 160 * 1024, "LDS of a compute unit, with the flags in front");
   auto kernel = packed_prompt_kernel<HD, SETS, EXTRA>;
   static bool raised[64] = {};                 // per instantiation and device
   int device = 0;
