@@ -35,3 +35,28 @@ def test_the_same_bits_beside_any_number_of_rows(ops, gpu_device, unit):
     want = ops.linear_silu_mul(x, weight, torch.float32, **unit)
     for rows in (1, 2, 5, 17, 64, 129):
         assert torch.equal(ops.linear_silu_mul(x[:rows].contiguous(), weight, torch.float32, **unit), want[:rows]), rows
+
+
+@pytest.mark.parametrize("unit", UNITS)
+@pytest.mark.parametrize("rows", [1, 3, 20, 100, 300])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_what_is_no_number_stays_so(ops, gpu_device, unit, rows, value):
+    """A row, or an output channel, with a NaN or an infinity gives NaN behind every unit, clamped ones too; the
+    others know nothing of it."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(rows, 640, generator=g).to(gpu_device)
+    w = (0.1 * torch.randn(2 * 96, 640, generator=g)).to(gpu_device)
+    want = ops.linear_silu_mul(x, ops.quantize_weight(w), torch.float32, **unit)
+    assert torch.isfinite(want).all()
+    bad = x.clone()
+    bad[rows // 2, 77] = value
+    got = ops.linear_silu_mul(bad, ops.quantize_weight(w), torch.float32, **unit)
+    keep = torch.arange(rows, device=gpu_device) != rows // 2
+    assert torch.equal(got[keep], want[keep]) and torch.isnan(got[rows // 2]).all()
+    assert torch.isnan(ops.linear(bad, ops.quantize_weight(w), torch.float32)[rows // 2]).all()
+    for channel in (5, 96 + 5):                       # of the gate, of the up rows
+        weight = w.clone()
+        weight[channel, 33] = value
+        got = ops.linear_silu_mul(x, ops.quantize_weight(weight), torch.float32, **unit)
+        others = torch.arange(96, device=gpu_device) != 5
+        assert torch.equal(got[:, others], want[:, others]) and torch.isnan(got[:, 5]).all()

@@ -9,9 +9,13 @@
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 
+// A scale as products take it: of a row with an infinity (an infinite scale, and numbers that say nothing) NaN, so that
+// what it gives is no number behind a clamp either.
+__device__ __forceinline__ float int8_scale(float s) { return s + (s - s); }
+
 // The gated unit of all these products: gated_unit's three forms in one, by the hardware's exp2 and reciprocal (an ulp each),
 // the same instructions whichever kernel a row's product comes from, so that its bits do not depend on the rows beside it.
-// (The clamps change nothing without a limit; a clamp takes NaN for its limit, as gated_unit's does.)
+// (The clamps change nothing without a limit, and NaN stays NaN.)
 struct Int8Unit {
   float top, lift, slope, cubic;
   __device__ __forceinline__ explicit Int8Unit(float limit) {
@@ -22,7 +26,8 @@ struct Int8Unit {
     cubic = gelu ? 0.044715f * slope : 0.f;
   }
   __device__ __forceinline__ float operator()(float gate, float up) const {
-    const float g = fminf(gate, top), u = fminf(fmaxf(up, -top), top) + lift;
+    const float g = __builtin_elementwise_minimum(gate, top);
+    const float u = __builtin_elementwise_minimum(__builtin_elementwise_maximum(up, -top), top) + lift;
     return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * fmaf(cubic, g * g, slope))) * u;
   }
 };

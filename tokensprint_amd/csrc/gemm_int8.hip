@@ -28,14 +28,14 @@ __device__ __forceinline__ void finish_few(const Int8Args& a, i32x4 (&acc)[HALVE
     for (int h = 0; h < HALVES; ++h) acc[h] += red[o][h][lane];
   const int n = n0 + lane / 16 * 4;
   if (n >= a.N || m >= a.M) return;
-  const float row = scales[m];
+  const float row = int8_scale(scales[m]);
   const Int8Unit unit(a.limit);
   f32x4 v;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int column = min(n + i, a.N - 1);
-    v[i] = (float)acc[0][i] * a.w_scale[column] * row;
-    if constexpr (PAIR) v[i] = unit(v[i], (float)acc[1][i] * a.w_scale[a.N + column] * row);
+    v[i] = (float)acc[0][i] * int8_scale(a.w_scale[column]) * row;
+    if constexpr (PAIR) v[i] = unit(v[i], (float)acc[1][i] * int8_scale(a.w_scale[a.N + column]) * row);
   }
   store4<TC>((TC*)a.c + (int64_t)m * a.N + n, v, a.N - n);
 }

@@ -680,10 +680,15 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
     }
     constexpr int COLS = PAIR ? TN / 2 : TN;
     const Int8Unit unit(g.limit);
+    float rows[TM];
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) rows[tm] = g.a_scale[min(m0 + wm * WM + tm * 16 + r, g.M - 1)];
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) rows[tm] = int8_scale(rows[tm]);
     auto scales = [&](const float* p, int n) {
       f32x4 s;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] = p[min(n + e, g.N - 1)];
+      for (int e = 0; e < 4; ++e) s[e] = int8_scale(p[min(n + e, g.N - 1)]);
       return s;
     };
 #pragma unroll
@@ -697,7 +702,7 @@ __global__ __launch_bounds__(64 * GM * GN, 1) void gemm_tiled_kernel(TiledArgsOf
       for (int tm = 0; tm < TM; ++tm) {
         const int m = m0 + wm * WM + tm * 16 + r;
         if (m >= g.M) continue;
-        const float row = g.a_scale[m];
+        const float row = rows[tm];
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

@@ -1,8 +1,8 @@
 // Rows in 8 bits: scale = the row's largest magnitude / 127, an element the nearest whole number of scales,
 // ties to even.  Alone (weights too: a row is an output channel), or behind the residual add and the RMSNorm
 // whose rows go into an 8-bit product: the normed row is quantised as it is in registers, never rounded to the activation
-// type or written in it.  A row with an infinity or a NaN has a scale that is neither finite, so its products
-// are not numbers either.
+// type or written in it.  A row with an infinity or a NaN has a scale that is neither finite, and its products
+// are NaN (int8_scale in gemm_int8.h).
 //
 // A workgroup takes a row, eight neighbouring elements a piece: bound by memory for many rows (8,192 of 5,120 28 us, 4.5
 // TB/s; with the add and the norm 87 us, 5.3 TB/s), by one trip and two meetings of the workgroup for few (3.3 us).  Codes go into rows of `row` bytes (a multiple of 256, zeros behind the
