@@ -60,3 +60,28 @@ def test_what_is_no_number_stays_so(ops, gpu_device, unit, rows, value):
         got = ops.linear_silu_mul(x, ops.quantize_weight(weight), torch.float32, **unit)
         others = torch.arange(96, device=gpu_device) != 5
         assert torch.equal(got[:, others], want[:, others]) and torch.isnan(got[:, 5]).all()
+
+
+@pytest.mark.parametrize("unit", UNITS)
+@pytest.mark.parametrize("rows", [1, 3, 20, 100, 300])
+def test_gates_whose_square_is_no_float32(ops, gpu_device, unit, rows):
+    """Gates of some 1e20 are finite, and so is what the unit makes of them: the unit's weight is 0 or 1 there."""
+    g = torch.Generator().manual_seed(6)
+    x = (4e19 * torch.randn(rows, 640, generator=g)).to(gpu_device)
+    gate, up = torch.randn(96, 640, generator=g), 1e-20 * torch.randn(96, 640, generator=g)
+    weight = ops.quantize_weight(torch.cat([gate, up]).to(gpu_device))
+    held = ops.quantize_rows(x)
+    sums = held.codes.double().cpu() @ weight.codes.double().cpu().T
+    y = sums * held.scales.double().cpu()[:, None] * weight.scales.double().cpu()
+    big, u = y[:, :96], y[:, 96:]
+    assert big.abs().max() > 2e19 and (big.abs() > 1e5).all()
+    if "limit" in unit:
+        want = torch.where(big > 0, 1.5 * torch.sigmoid(torch.tensor(1.5 * 1.702).double()), 0.0) * (u.clamp(-1.5, 1.5) + 1)
+    else:
+        want = big.clamp(min=0) * u
+    got = ops.linear_silu_mul(x, weight, torch.float32, **unit).double().cpu()
+    # two roundings for each of the two products' results, an ulp each of exp2 and reciprocal (and half a one of its
+    # argument, 3.7 at the most in units of log2, times ln 2), the sums and products of the unit: below 16 halves of an ulp;
+    # where u + 1 cancels, u's share of that
+    bound = 2.0 ** -20 * (want.abs() + torch.where(big > 0, 2.0, 0.0)) if "limit" in unit else 2.0 ** -20 * want.abs()
+    assert bool(((got - want).abs() <= bound).all())

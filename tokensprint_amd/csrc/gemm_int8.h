@@ -28,7 +28,9 @@ struct Int8Unit {
   __device__ __forceinline__ float operator()(float gate, float up) const {
     const float g = __builtin_elementwise_minimum(gate, top);
     const float u = __builtin_elementwise_minimum(__builtin_elementwise_maximum(up, -top), top) + lift;
-    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * fmaf(cubic, g * g, slope))) * u;
+    // (from 10^4 on the weight is 0 or 1; a gate of 2e19 has no square, and 0 times that is no number)
+    const float e = __builtin_amdgcn_fmed3f(g, -1e4f, 1e4f);
+    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e * fmaf(cubic, e * e, slope))) * u;
   }
 };
 
