@@ -155,22 +155,23 @@ class Dispatch:
     # key/value head) and one key/value head; us with 8 key/value heads of 128, pages of 16.
     #: steps of up to this many items are one launch, portions of prompts among them; above it
     #: portions have the kernel that makes tiles in LDS for 128 rows (a prompt of 500 tokens of 16
-    #: heads, 504 items: 16 / 18; of 32 heads, 1,000 items: 29 / 18; 500 tokens behind 2,000: 43 / 54 and
-    #: 82 / 55; 30 single tokens beside 200 behind 2,000 of 16 heads: 37 / 68)
+    #: heads, 504 items: 16 / 19; of 32 heads, 1,000 items: 30 / 19; 500 tokens behind 2,000: 43 / 56 and
+    #: 81 / 56; 30 single tokens beside 200 behind 2,000 of 16 heads: 37 / 69)
     packed_few: int = 512
     #: tokens from which a portion counts as one there (8 portions of 16 tokens behind 500 are
-    #: 10 as items and 19 in tiles, but 512 items of portions of 64 tokens and more 20 and 20, 1,024 36 and 21)
+    #: 10 as items and 20 in tiles, but 512 items of portions of 64 tokens 20 and 21, 1,024 of 128 36 and 22)
     packed_portion: int = 16
     #: up to this many items a workgroup each (or their keys shared out, see the next), above it a
-    #: wavefront each (single tokens: 128 requests of 100 to 3,000 tokens, 1,024 items, 68 / 92; of 500, 32 /
-    #: 22; 160 requests of 100 to 3,000 98 / 114, of 500 39 / 31, 256 of 4,000 260 / 223; prompts of 4,000 tokens in
-    #: float32, 4,000 items, 361 / 243)
+    #: wavefront each (single tokens: 128 requests of 100 to 3,000 tokens, 1,024 items, 72 / 96; of 500, 32 /
+    #: 22; 160 requests of 100 to 3,000 102 / 116, of 500 38 / 31; 256 of 100 to 3,000 138 / 123, of 4,000 249 / 212;
+    #: prompts of 4,000 tokens in float32, 4,000 items, 450 / 250.  The count is no measure of one request far longer than
+    #: the others: 128 of 500 and one of 30,000 48 / 917)
     packed_items: int = 1024
     #: contexts of up to this many tokens are a workgroup per item without a look at the lengths; longer
-    #: ones are shared out where the lengths on the device say so (1 request of 1,000: 9.7 whole, 11.5 with the
-    #: look; of 2,000 15 / 11; of 8,000 46 / 14; 4 requests of 1,300 12 / 14, of 2,500 18 / 13)
+    #: ones are shared out where the lengths on the device say so (1 request of 1,000: 9.9 whole, 11.4 with the
+    #: look; of 2,000 16 / 11; of 8,000 46 / 14; 4 requests of 1,300 12 / 14, of 2,500 18 / 12)
     packed_whole: int = 1280
-    #: the same for 1,024 items, which take turns (128 requests of 4,000: 121 / 130; of 1,300 52 / 59)
+    #: the same for 1,024 items, which take turns (128 requests of 4,000: 121 / 127; of 1,300 52 / 59)
     packed_whole_many: int = 4096
     #: workgroups that keys are shared out over; 0: one for each compute unit
     packed_workgroups: int = 0
