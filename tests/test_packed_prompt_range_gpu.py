@@ -149,3 +149,22 @@ def test_values_of_many_sizes_in_one_context(ops, gpu_device, hd, order, sets):
     # a third of that as the deviation of all of them, twice that is allowed)
     worst = relative(got, want)
     assert worst <= TOLERANCE[BF16] + 2.0 ** -7 * 2 / 3
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("sets", [1, 2])
+@pytest.mark.parametrize("size,place", [(40.0, 33), (40.0, 2500), (1500.0, 33)])
+def test_a_large_value_that_counts_little(ops, gpu_device, hd, sets, size, place):
+    """A key far above the rest, and one far below it with values a thousand times the others' and more: the others, which
+    are what the result is made of, keep the bits of their weights."""
+    spans = [(3000, 24), (2600, 17)] if sets == 2 else [(2600 + i, 1) for i in range(130)]
+    args = list(peaked(gpu_device, BF16, nq=4, nkv=2, hd=hd, spans=spans, above=14.0625, std=0.05, place=0))
+    first = 0
+    for n in args[4].q_lens:
+        args[1][first + place, :, 0] = -14.0
+        args[2][first + place] = (rand((2, hd), F32, gpu_device, 12 + first) * size).to(BF16)
+        first += n
+    got, want = run(ops, *args)
+    # (2,600 others of 0.05 and weights around e: some 5 in all; that key's 1,500 e^-14 is 0.0012)
+    worst = relative(got, want)
+    assert worst <= TOLERANCE[BF16]

@@ -12,21 +12,23 @@
 // The next turn's codes, asked for a turn ahead, become numbers between the scores' products, a word a step, and the second
 // half of a turn's weights are made between the first half's products: a turn is one meeting of the workgroup.
 // 4,096 tokens behind 4,096, 32 heads of 128 over 8: 475 to 495 us by card, 835 to 870 TFLOP/s (all codes of a turn first, then
-// its products: 0.6 % longer; over a cache of bfloat16 a tenth shorter), vector instructions three quarters of the time and
-// matrix instructions 40 %.
+// its products: 0.6 % longer; over a cache of bfloat16 a tenth shorter), vector instructions 60 % of a SIMD's cycles and
+// matrix instructions 37 %.
 #pragma once
 #include "attention_prefill_tall_kernel.h"
 #include "packed_attention_kernel.h"
 
-// What a block's numbers count: values 2^11 times where its largest step is below 2, else 2^-4, keys 2^4 times below 256,
-// else 2^-4: 15 steps stay below float16's largest number, and a step of float16's smallest has 11 bits in a block of the
-// first kind (in one of the second numbers are held to 2^-21).  Nearly every block is of the first; one of the second is
-// told to the workgroup beside the tile, and the scores and weights of a turn with such a block make up for it.
+// What a block's numbers count: values 2^11 times where its largest step is below 2, 2^(11 - n) times where it is below
+// 2^(1 + n), n up to 15, keys 2^4 times below 256, else 2^-4: 15 steps stay below float16's largest number, and a step of
+// float16's smallest has 11 bits in an ordinary block (in another, values are held to 2^(n - 36), large keys to 2^-21).
+// Nearly every block is ordinary; another is told to the workgroup beside the tile, and the scores and weights of a turn with
+// such a block make up for it: from there on the weights of ordinary blocks count 2^n times less, and have 11 bits down to
+// 2^(n - 29) of the row's largest.
 // (A sixteenth for all, the most that holds the largest step, took 1.7 % less time and left numbers below 2^-10 without all
 // their bits: values of 1e-4 came out 0.3 % off, of 1e-5 3 %.)
 struct PromptScale {
-  static constexpr int kValues = 11, kKeys = 4, kLarge = -4;
-  static constexpr int kLargeValues = 1, kLargeKeys = 2;               // a block's flags
+  static constexpr int kKeys = 4, kValues = 11;
+  static constexpr int kLargeKeys = 1, kValuesDown = 2;                // a block's flags: of its keys, and n times the other
 };
 
 // Tiles and operands lie as there. SETS sets of four wavefronts split an item's turns and merge through LDS at the end.
@@ -165,9 +167,18 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
     for (int i = 0; i < PG; ++i) ks[i] = held + r16 <= pos_last ? ks[i] : 0u;
   };
+  // The values' n, ahead of a turn, so that another than 0 is a branch's.
+  const unsigned step_lanes = lane % 4 < 2 ? 0x40004000u : 0u;         // bit 14: 2 and more
+  int down = 0;
+  auto look = [&]() {
+    down = 0;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64((vs & step_lanes) != 0) == 0, 1)) return;
+    asm volatile("" ::: "memory");             // keeps this a branch
+    const unsigned exponent = step_lanes != 0 ? max(vs >> 10 & 31u, vs >> 26 & 31u) : 0u;
+    down = uniform((int)wave_max((float)exponent)) - 15;
+  };
   // Steps as the numbers want them, keys', then values', and the block's flags.  (Without a branch, which would end the
   // stretch in which the compiler may order products and these.)
-  const unsigned step_lanes = lane % 4 < 2 ? 0x40004000u : 0u;         // bit 14: 2 and more
   int flags_now = 0, told = 0;
   // (of their own: in the registers that loads go to, they would make the next turn's be waited for)
   _Float16 key_step[PG];
@@ -184,9 +195,9 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
       key_step[i] = __builtin_bit_cast(_Float16, (unsigned short)ks[i]) * up;
   };
   auto scale_values = [&]() {
-    const bool large = __builtin_amdgcn_ballot_w64((vs & step_lanes) != 0) != 0;
-    flags_now += large ? PromptScale::kLargeValues : 0;
-    const unsigned up = step_lanes != 0 ? (large ? 0x2c002c00u : 0x68006800u) : 0x3c003c00u;
+    flags_now += PromptScale::kValuesDown * down;
+    const unsigned by = (unsigned)(15 + PromptScale::kValues - down) * 0x04000400u;
+    const unsigned up = step_lanes != 0 ? by : 0x3c003c00u;
     value_steps = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, vs) * __builtin_bit_cast(f16x2, up));
   };
   // (a wavefront that has told of a block once does so for all that follow, so that what stands there is this turn's)
@@ -349,7 +360,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
       int up[G], least = up_o;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        up[g] = uniform(flags[g]) & PromptScale::kLargeValues ? PromptScale::kLarge : PromptScale::kValues;
+        up[g] = PromptScale::kValues - uniform(flags[g]) / PromptScale::kValuesDown;
         least = min(least, up[g]);
       }
       if (least != up_o) {
@@ -409,6 +420,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
   if (mine > 0) {
     issue(0);
     if (held + 15 > pos_last) mask_steps();
+    look();
     unpack_all(ring);
     tell(s_flags[set][0]);
     if (mine > 1) issue(1);
@@ -418,6 +430,7 @@ __global__ __launch_bounds__(256 * SETS) __attribute__((amdgpu_waves_per_eu(2, 2
     const int kb = walk.real(kb_first + KEYS * SETS * j);
     unsigned char *buf = ring + (j & 1) * BUF, *next = ring + (~j & 1) * BUF;
     if (j + 1 < mine && held + 15 > pos_last) mask_steps();
+    look();
     // (behind the last turn what is left in the registers once more, into a tile that nobody reads)
     const bool seen = kb <= tile_last && (kb + KEYS - 1 >= tile_lo || kb < a.keep);
     if (j < mine && !seen) {
