@@ -12,8 +12,8 @@
 // The next turn's codes, asked for a turn ahead, become numbers between the scores' products, a word a step, and the second
 // half of a turn's weights are made between the first half's products: a turn is one meeting of the workgroup.
 // 4,096 tokens behind 4,096, 32 heads of 128 over 8: 475 to 495 us by card, 835 to 870 TFLOP/s (all codes of a turn first, then
-// its products: 0.6 % longer; over a cache of bfloat16 a tenth shorter), vector instructions 60 % of a SIMD's cycles and
-// matrix instructions 37 %.
+// its products: 0.6 % longer; over a cache of bfloat16 a tenth shorter), vector instructions 59 % of a SIMD's cycles and
+// matrix instructions 36 %.
 #pragma once
 #include "attention_prefill_tall_kernel.h"
 #include "packed_attention_kernel.h"
