@@ -137,10 +137,10 @@ class _PendingMerge:
     """A decode step's attention output that still lies in the partial results of its key
     splits: `out` is where the merge puts it.  Holds the partial results alive."""
 
-    def __init__(self, ops, out, args, partial_o, partial_ml, positions, window):
+    def __init__(self, ops, out, args, partial_o, partial_ml, positions):
         self.ops, self.out, self.args = ops, out, args       # args: AttentionMfmaArgs
         self.partial_o, self.partial_ml = partial_o, partial_ml
-        self.positions, self.window = positions, window
+        self.positions = positions
         self.done = False
 
     def merge(self) -> None:
@@ -675,8 +675,7 @@ class HipOps:
         self._call(self.lib.ts_gemm_tail_merged_bf16, _ptr(unmerged.partial_o),
                    _ptr(unmerged.partial_ml), _ptr(unmerged.positions),
                    unmerged.args.num_splits, a.nq, a.nkv, a.hd,
-                   0 if unmerged.window is None else int(unmerged.window), _ptr(weight),
-                   _ptr(resid), _ptr(hint.norm_weight), _ptr(rows), _ptr(sumsq), M, N,
+                   a.window, _ptr(weight), _ptr(resid), _ptr(hint.norm_weight), _ptr(rows), _ptr(sumsq), M, N,
                    self._stream())
         return PreparedRows(rows, sumsq, parts, hint)
 
@@ -1370,10 +1369,10 @@ class HipOps:
         d.cos, d.sin, d.eps, d.kv_in_row = qa.cos, qa.sin, eps, kv_in_row
         d.row_extra = row_extra
         pending = self._attention_decode(a, batch, num_heads // num_kv_heads, d,
-                                         out if defer_merge else None, window)
+                                         out if defer_merge else None)
         return out if pending is None else UnmergedRows(pending, out.shape)
 
-    def _attention_decode(self, a, batch, group, d=None, defer_out=None, window=None):
+    def _attention_decode(self, a, batch, group, d=None, defer_out=None):
         """One token per entry: workgroups per (entry, key/value head, share of the keys).
         `defer_out`: the output tensor, if the merge of the splits may be left undone; then
         the pending merge is returned (else None)."""
@@ -1400,7 +1399,7 @@ class HipOps:
         self._call(self.lib.ts_attention_decode, byref(d), self._stream())
         if d.defer_merge:
             kept = AttentionMfmaArgs.from_buffer_copy(m)
-            return _PendingMerge(self, defer_out, kept, po, pml, batch.positions, window)
+            return _PendingMerge(self, defer_out, kept, po, pml, batch.positions)
         return None
 
     def _decode_fits(self, batch, num_kv_heads, group, head_dim, page_size, fused):
