@@ -1,3 +1,4 @@
+import gc
 import sys
 from pathlib import Path
 
@@ -18,3 +19,11 @@ def gpu_device():
     if not torch.cuda.is_available():
         pytest.skip("no GPU")
     return torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def garbage_of_earlier_modules():
+    """What earlier modules' tests left in reference cycles is freed before a module begins, not
+    whenever Python next looks for it: a test that reads the device's memory before and after a
+    call must not find an earlier test's tensors freed in between."""
+    gc.collect()
